@@ -19,7 +19,7 @@
 //             one texel's CP*4 contiguous bytes; texels outside the map and
 //             lanes that do not need the view carry an out-of-range offset,
 //             which the buffer hardware answers with 0 and no memory traffic.
-//   mix       bilinear mix (packed fp32) and view sum in registers.
+//   mix       bilinear mix and view sum in registers.
 //   The loop is software-pipelined inside the wave: fetches of view s fly under
 //   the projection of view s+1.
 // Then: normalise (exact division by count + 1e-6), clamp, transpose through
@@ -644,7 +644,7 @@ __device__ __forceinline__ void unproject_wave(const UnprojArgs& a, int b, int f
           const int vsl = s * VPS + vq;
           const int rd = (lane_on && vsl < kWaveVox) ? vsl : 0;
           const float4 w = s_wt[buf * kWaveVox + rd];
-          // channels 4cq..4cq+3 as two packed pairs; same chain as
+          // channels 4cq..4cq+3 as two pairs; same chain as
           // tempo_bilinear_mix, then the view sum
           const f32x2 a01 = {__uint_as_float(tex[g][0][0]), __uint_as_float(tex[g][0][1])};
           const f32x2 a23 = {__uint_as_float(tex[g][0][2]), __uint_as_float(tex[g][0][3])};

@@ -57,8 +57,8 @@ enum { TEMPO_UNFUSED_R = 1, TEMPO_UNFUSED_K = 2, TEMPO_UNFUSED_A = 4, TEMPO_UNFU
 #endif
 
 // ---- pairs: the x and y coordinate go through identical operation chains, so
-// they are carried as 2-vectors; on gfx950 these become packed-fp32 VALU ops
-// (v_pk_mul/add/fma_f32: two lanes' worth per issue slot)
+// they are carried as 2-vectors (the build keeps the compiler from turning these
+// into packed-fp32 instructions, see build.py)
 #if defined(__HIPCC__)
 typedef float tempo_f2 __attribute__((ext_vector_type(2)));
 #define TEMPO_FMA2(a, b, c) __builtin_elementwise_fma((a), (b), (c))
