@@ -48,7 +48,7 @@
 extern "C" {
 #endif
 
-#define TEMPO_ABI_VERSION 14
+#define TEMPO_ABI_VERSION 15
 #define TEMPO_CAM_FLOATS 32
 #define TEMPO_MAX_VIEWS 32
 #define TEMPO_MAX_CHANNELS 32 /* per call; wider tensors go in channel slices */
@@ -56,7 +56,9 @@ extern "C" {
 #define TEMPO_STATIC_SCRATCH_BYTES (64u << 20)
 #define TEMPO_MM_FMA 0
 #define TEMPO_MM_UNFUSED 7
-/* element types of tempo_repack_nhwc_half's inputs */
+/* tempo_recurrence stores the state in front of every TEMPO_RECURRENCE_SPAN-th step */
+#define TEMPO_RECURRENCE_SPAN 16
+/* element types of tempo_repack_nhwc_half's inputs and of the temporal head's tensors */
 #define TEMPO_DTYPE_F32 0
 #define TEMPO_DTYPE_F16 1
 #define TEMPO_DTYPE_BF16 2
@@ -553,6 +555,42 @@ int tempo_project_points(const float* pts, const float* cam, int M, int N,
                          float hm_w, float hm_h, float img_w, float img_h,
                          int mm_unfused, float* pix, float* grid, uint8_t* inside,
                          void* stream);
+
+/* Gated linear recurrence over time -- the update of the reference's temporal cell
+ * (SpatialGRU, fiery_temporal.py:109) with gates that depend on the input alone:
+ *   z = sigmoid(gate[b, t, :]);  h[b, t] = (1 - z) h[b, t-1] + z value[b, t]
+ * for t < len(b), h[b, -1] = state[b].  Rows t >= len(b) of gate and value are not read and
+ * those of h are zeroed.
+ *   gate, value, h : element type `dtype` (TEMPO_DTYPE_*), element (b, t, d) at
+ *            b * <name>_sb + t * <name>_st + d (strides in elements, channels adjacent)
+ *   state  : fp32 [B, D] or NULL (zeros);  lengths : int32 [B] or NULL (all T; values
+ *            outside [0, T] count as the nearer end)
+ *   last   : fp32 [B, D] or NULL: the state after the last step; may be `state` itself
+ *   ckpt   : fp32 [ceil(T / TEMPO_RECURRENCE_SPAN), B, D] or NULL: states for the backward
+ *            pass (T <= TEMPO_RECURRENCE_SPAN: not needed, `state` serves as ckpt there)
+ *   workspace : tempo_recurrence_workspace(B, T, D, dtype, 0) bytes, 4-byte aligned (a
+ *            negative value is a TEMPO_E_* code); not shared by calls that overlap in time
+ * Sums and states are fp32; no atomics: results do not change from run to run.
+ *
+ * tempo_recurrence_backward: from grad_h (dtype) and grad_last (fp32 [B, D] or NULL, zeros)
+ * to grad_gate, grad_value (dtype; rows t >= len(b) are zeroed) and grad_state (fp32 [B, D] or
+ * NULL).  ckpt is what the forward wrote; NULL stands for zeros where T <= the span.
+ * workspace : tempo_recurrence_workspace(B, T, D, dtype, 1) bytes. */
+long long tempo_recurrence_workspace(long long B, int T, int D, int dtype, int backward);
+int tempo_recurrence(const void* gate, long long gate_sb, long long gate_st,
+                     const void* value, long long value_sb, long long value_st,
+                     const float* state, const int32_t* lengths, void* h, long long h_sb,
+                     long long h_st, float* last, float* ckpt, long long B, int T, int D,
+                     int dtype, void* workspace, long long workspace_bytes, void* stream);
+int tempo_recurrence_backward(const void* gate, long long gate_sb, long long gate_st,
+                              const void* value, long long value_sb, long long value_st,
+                              const void* grad_h, long long grad_sb, long long grad_st,
+                              const float* grad_last, const int32_t* lengths,
+                              const float* ckpt, void* grad_gate, long long dgate_sb,
+                              long long dgate_st, void* grad_value, long long dvalue_sb,
+                              long long dvalue_st, float* grad_state, long long B, int T,
+                              int D, int dtype, void* workspace, long long workspace_bytes,
+                              void* stream);
 
 #ifdef __cplusplus
 }

@@ -9,9 +9,11 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get('TEMPO_LIB') or os.path.join(_HERE, 'lib', 'libtempo_unproject.so')
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _c_void_p, _c_int, _c_float = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+_c_ll = ctypes.c_longlong
+_strided = [_c_void_p, _c_ll, _c_ll]  # pointer, batch stride, time stride
 
 # name -> (restype, argtypes); mirrors include/tempo_unproject.h one to one
 SIGNATURES = {
@@ -93,6 +95,12 @@ SIGNATURES = {
                               [_c_int] * 6 + [_c_void_p] * 6),
     'tempo_project_points': (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int] +
                              [_c_float] * 4 + [_c_int] + [_c_void_p] * 4),
+    'tempo_recurrence_workspace': (_c_ll, [_c_ll] + [_c_int] * 4),
+    'tempo_recurrence': (_c_int, _strided * 2 + [_c_void_p] * 2 + _strided + [_c_void_p] * 2 +
+                         [_c_ll] + [_c_int] * 3 + [_c_void_p, _c_ll, _c_void_p]),
+    'tempo_recurrence_backward': (_c_int, _strided * 3 + [_c_void_p] * 3 + _strided * 2 +
+                                  [_c_void_p, _c_ll] + [_c_int] * 3 +
+                                  [_c_void_p, _c_ll, _c_void_p]),
 }
 
 _lib = None

@@ -24,6 +24,7 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall',
 # source -> (what it includes, flags of its own)
 SOURCES = {
     'tempo_unproject.hip': (['unproject_math.h'], ['-ffp-contract=off']),
+    'recurrence.hip': ([], []),
 }
 
 

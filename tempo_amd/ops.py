@@ -1246,3 +1246,160 @@ def window_geometry(grid_center, scale, bias, space_size, sub_space_size, fine_b
                                        _ptr(live), _stream_ptr(dev))
     _lib.check(rc, 'tempo_window_geometry')
     return tl, offset, start, end, live
+
+
+# --------------------------------------------------------------------------
+# temporal head: gated linear recurrence
+# --------------------------------------------------------------------------
+
+RECURRENCE_SPAN = 16  # TEMPO_RECURRENCE_SPAN: steps between stored states
+FLOAT_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}  # TEMPO_DTYPE_*
+
+
+def _float_tensor(t, name, dim, dtype=None, device=None):
+    """A ``dim``-dimensional fp32 / fp16 / bf16 tensor on a HIP device with adjacent channels."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f'{name}: expected a tensor on a HIP device (tempo_amd has no CPU path)')
+    if t.dtype not in FLOAT_DTYPES or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f'{name}: expected {dtype or "float32, float16 or bfloat16"}, '
+                        f'got {t.dtype}')
+    if device is not None and t.device != device:
+        raise ValueError(f'{name}: on {t.device}, expected {device}')
+    if t.dim() != dim:
+        raise ValueError(f'{name}: expected {dim} dimensions, got {tuple(t.shape)}')
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f'{name}: the channels (last dimension) must be adjacent in memory')
+    return t
+
+
+def _strided(t):
+    return _ptr(t), t.stride(0), t.stride(1)
+
+
+def _like_time_order(t, channels):
+    """Empty ``[B,T,channels]`` whose memory has time outermost where ``t``'s has."""
+    B, T, _ = t.shape
+    if B > 1 and T > 1 and t.stride(1) > t.stride(0):
+        return torch.empty(T, B, channels, dtype=t.dtype, device=t.device).transpose(0, 1)
+    return torch.empty(B, T, channels, dtype=t.dtype, device=t.device)
+
+
+def _recurrence_inputs(gate, value, lengths):
+    _float_tensor(gate, 'gate', 3)
+    if value is None:
+        if gate.shape[2] % 2:
+            raise ValueError('gate: without a value its channels are gate and value side by '
+                             'side, an even number')
+        D = gate.shape[2] // 2
+        gate, value = gate[..., :D], gate[..., D:]
+    else:
+        _float_tensor(value, 'value', 3, gate.dtype, gate.device)
+        if value.shape != gate.shape:
+            raise ValueError(f'value: {tuple(value.shape)}, gate: {tuple(gate.shape)}')
+    B, T, D = (int(n) for n in gate.shape)
+    if D == 0:
+        raise ValueError('gate: no channels')
+    if lengths is not None:
+        _need(lengths, torch.int32, 'lengths', gate.device)
+        if tuple(lengths.shape) != (B,):
+            raise ValueError(f'lengths: expected [{B}], got {tuple(lengths.shape)}')
+    return gate, value, B, T, D
+
+
+def _lane_state(t, name, B, D, dev):
+    if t is not None:
+        _need(t, torch.float32, name, dev)
+        if tuple(t.shape) != (B, D):
+            raise ValueError(f'{name}: expected [{B},{D}], got {tuple(t.shape)}')
+    return t
+
+
+def _workspace(bytes_, what, dev):
+    """Scratch memory of one call.  From torch's allocator every time: its blocks follow the
+    stream (and, under capture, belong to the graph), so no two calls share one."""
+    if bytes_ < 0:
+        _lib.check(int(bytes_), what)
+    return torch.empty((bytes_ + 3) // 4, dtype=torch.float32, device=dev) if bytes_ else None
+
+
+def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, state_out=None,
+                       want_ckpt=False):
+    """``h_t = (1 - z_t) h_{t-1} + z_t v_t``, ``z = sigmoid(gate)`` -> ``(h, last, ckpt)``;
+    arguments as :func:`tempo_amd.gated_recurrence`.  ``ckpt``: the fp32 states in front of
+    every ``RECURRENCE_SPAN``-th step, which :func:`recurrence_backward` starts from (None
+    where ``T <= RECURRENCE_SPAN``: there ``state`` is all it needs)."""
+    lib = _lib.load()
+    _no_grad_path('recurrence_forward', gate, value, state)
+    gate, value, B, T, D = _recurrence_inputs(gate, value, lengths)
+    dev = gate.device
+    _lane_state(state, 'state', B, D, dev)
+    if out is None:
+        out = _like_time_order(gate, D)
+    else:
+        _float_tensor(out, 'out', 3, gate.dtype, dev)
+        if out.shape != gate.shape:
+            raise ValueError(f'out: expected {tuple(gate.shape)}, got {tuple(out.shape)}')
+    last = _lane_state(state_out, 'state_out', B, D, dev)
+    if last is None:
+        last = torch.empty(B, D, dtype=torch.float32, device=dev)
+    if B == 0 or T == 0:
+        if last is not state:
+            last.copy_(state) if state is not None else last.zero_()
+        return out, last, None
+    ckpt = None
+    if want_ckpt and T > RECURRENCE_SPAN:
+        ckpt = torch.empty(-(-T // RECURRENCE_SPAN), B, D, dtype=torch.float32, device=dev)
+    code = FLOAT_DTYPES[gate.dtype]
+    with torch.cuda.device(dev):
+        need = lib.tempo_recurrence_workspace(B, T, D, code, 0)
+        ws = _workspace(need, 'tempo_recurrence_workspace', dev)
+        rc = lib.tempo_recurrence(*_strided(gate), *_strided(value), _ptr(state), _ptr(lengths),
+                                  *_strided(out), _ptr(last), _ptr(ckpt), B, T, D, code,
+                                  _ptr(ws), need, _stream_ptr(dev))
+    _lib.check(rc, 'tempo_recurrence')
+    return out, last, ckpt
+
+
+def recurrence_backward(grad_h, grad_last, gate, value=None, state=None, ckpt=None,
+                        lengths=None, want_state=False):
+    """Gradients of :func:`recurrence_forward`: ``(grad_gate, grad_value, grad_state)``;
+    ``grad_value`` is None where gate and value came side by side (``grad_gate`` holds both).
+    ``grad_h`` / ``grad_last`` None: zeros."""
+    lib = _lib.load()
+    both = value is None
+    packed = gate
+    gate, value, B, T, D = _recurrence_inputs(gate, value, lengths)
+    dev = gate.device
+    if grad_h is None:
+        grad_h = torch.zeros(D, dtype=gate.dtype, device=dev).expand(B, T, D)
+    elif D > 1 and grad_h.stride(-1) != 1:
+        grad_h = grad_h.contiguous()
+    _float_tensor(grad_h, 'grad_h', 3, gate.dtype, dev)
+    if grad_h.shape != gate.shape:
+        raise ValueError(f'grad_h: expected {tuple(gate.shape)}, got {tuple(grad_h.shape)}')
+    _lane_state(grad_last, 'grad_last', B, D, dev)
+    _lane_state(state, 'state', B, D, dev)
+    if T > RECURRENCE_SPAN and B:
+        _need(ckpt, torch.float32, 'ckpt', dev)
+        if tuple(ckpt.shape) != (-(-T // RECURRENCE_SPAN), B, D):
+            raise ValueError('ckpt has the wrong size')
+    else:
+        ckpt = state
+    dpacked = _like_time_order(packed, int(packed.shape[2]))
+    dgate, dvalue = (dpacked[..., :D], dpacked[..., D:]) if both else \
+        (dpacked, _like_time_order(gate, D))
+    dstate = torch.empty(B, D, dtype=torch.float32, device=dev) if want_state else None
+    if B == 0 or T == 0:
+        if want_state:
+            dstate.copy_(grad_last) if grad_last is not None else dstate.zero_()
+    else:
+        code = FLOAT_DTYPES[gate.dtype]
+        with torch.cuda.device(dev):
+            need = lib.tempo_recurrence_workspace(B, T, D, code, 1)
+            ws = _workspace(need, 'tempo_recurrence_workspace', dev)
+            rc = lib.tempo_recurrence_backward(
+                *_strided(gate), *_strided(value), *_strided(grad_h), _ptr(grad_last),
+                _ptr(lengths), _ptr(ckpt), *_strided(dgate), *_strided(dvalue), _ptr(dstate),
+                B, T, D, code, _ptr(ws), need, _stream_ptr(dev))
+        _lib.check(rc, 'tempo_recurrence_backward')
+    return dpacked, None if both else dvalue, dstate

@@ -1,0 +1,72 @@
+"""Differentiable operators of a temporal head on channel-last features.
+
+The reference carries features over time with a GRU (``tempo/models/fiery_temporal.py:109``,
+used at ``tempo/models/model_utils.py:10-16``), one step after the other.  Here the gates depend
+on the input alone, so that the recurrence is linear and runs over a whole sequence in one pass.
+
+Everything runs in HIP kernels on the current stream; there is no CPU path.  The backward
+passes use no atomics: gradients do not change from run to run.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def _records(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+class _GatedRecurrence(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, gate, value, state, lengths):
+        h, last, ckpt = ops.recurrence_forward(gate, value, state, lengths, want_ckpt=True)
+        # beyond one span the stored states replace the initial one
+        ctx.save_for_backward(gate, value, state if ckpt is None else None, ckpt, lengths)
+        ctx.set_materialize_grads(False)
+        return h, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_last):
+        if grad_h is None and grad_last is None:
+            return None, None, None, None
+        gate, value, state, ckpt, lengths = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if grad_last is not None:
+            grad_last = grad_last.contiguous()
+        dgate, dvalue, dstate = ops.recurrence_backward(grad_h, grad_last, gate, value, state,
+                                                        ckpt, lengths, want_state=need[2])
+        return (dgate if need[0] else None, dvalue if need[1] else None,
+                dstate if need[2] else None, None)
+
+
+def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state_out=None):
+    """Gated linear recurrence over time, ``h_t = (1 - z_t) h_{t-1} + z_t v_t`` with
+    ``z = sigmoid(gate)``: a GRU's update with gates from the input alone.
+
+    ``gate``, ``value``: ``[B,T,D]`` in fp32, fp16 or bf16, channels adjacent, any strides over
+    B and T (a transposed ``[T,B,D]`` tensor is read where it lies).  Without ``value``,
+    ``gate`` is ``[B,T,2D]`` with gate and value side by side, as one product leaves them.
+    ``state``: fp32 ``[B,D]``, the state before the first step (default: zeros).
+    ``lengths``: int32 ``[B]`` on the device; rows ``t >= lengths[b]`` are padding: not read,
+    0 in the result and in the gradients (values outside ``[0,T]`` count as the nearer end).
+
+    Returns ``(h [B,T,D], last [B,D])``: every state in the inputs' type and the fp32 state
+    after the last step, to go on from (a serving loop passes T = 1 and the carried state).
+    Differentiable once, with respect to ``gate``, ``value`` and ``state``.  States and sums are
+    fp32.  An infinity among the inputs leaves its channel's later states infinite or NaN.
+
+    ``out`` / ``state_out`` (not under autograd): where to write the two results;
+    ``state_out`` may be ``state`` itself.
+
+    To capture a training step into a graph, drop eager results of the same leaves first: torch
+    itself ends the process when a captured backward meets their gradient accumulators."""
+    if _records(gate, value, state):
+        if out is not None or state_out is not None:
+            raise NotImplementedError('gated_recurrence: out / state_out are for calls without '
+                                      'gradients (torch.no_grad() or detached tensors)')
+        return _GatedRecurrence.apply(gate, value, state, lengths)
+    h, last, _ = ops.recurrence_forward(gate, value, state, lengths, out, state_out)
+    return h, last
