@@ -62,6 +62,13 @@ extern "C" {
 #define TEMPO_DTYPE_F32 0
 #define TEMPO_DTYPE_F16 1
 #define TEMPO_DTYPE_BF16 2
+/* activations of tempo_linear; GELU is z * Phi(z) with the normal distribution itself */
+#define TEMPO_ACT_NONE 0
+#define TEMPO_ACT_RELU 1
+#define TEMPO_ACT_SILU 2
+#define TEMPO_ACT_GELU 3
+#define TEMPO_ACT_SIGMOID 4
+#define TEMPO_ACT_TANH 5
 
 enum {
   TEMPO_OK = 0,
@@ -591,6 +598,34 @@ int tempo_recurrence_backward(const void* gate, long long gate_sb, long long gat
                               long long dvalue_st, float* grad_state, long long B, int T,
                               int D, int dtype, void* workspace, long long workspace_bytes,
                               void* stream);
+
+/* Fused linear layer -- nn.Conv2d(K, N, 1) on channel-last rows (process_layer,
+ * rnn_multiview_pose.py:61-66) with its epilogue:
+ *   z = x W^T + bias;  y = act(z) + residual
+ *   x [M, K], weight [N, K], bias [N] or NULL, residual [M, N] or NULL, y [M, N], all of
+ *   element type `dtype`; ld* are the elements between rows (channels adjacent; rows of x,
+ *   weight and residual may coincide)
+ *   pre       : z as the backward pass needs it, contiguous [M, N], or NULL
+ *   workspace : tempo_linear_workspace(M, N, K, dtype, activation, 0) bytes, 16-byte aligned
+ *               (a negative value is a TEMPO_E_* code); not shared by calls that overlap in time
+ * Products and sums are fp32 throughout (fp32 inputs on fp32 matrix instructions), y is
+ * rounded once; no atomics: results do not change from run to run.
+ *
+ * tempo_linear_backward: dz = grad_y * act'(z); grad_x [M, K] = dz W, grad_weight [N, K]
+ * contiguous = dz^T x, grad_bias [N] = sum of dz over the rows; each NULL if not wanted (the
+ * residual's gradient is grad_y).  pre: what the forward wrote, NULL for TEMPO_ACT_NONE.
+ *   workspace : tempo_linear_workspace(..., 1) bytes. */
+long long tempo_linear_workspace(long long M, int N, int K, int dtype, int activation,
+                                 int backward);
+int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw,
+                 const void* bias, const void* residual, long long ldr, void* y,
+                 long long ldy, void* pre, long long M, int N, int K, int dtype,
+                 int activation, void* workspace, long long workspace_bytes, void* stream);
+int tempo_linear_backward(const void* grad_y, long long ldg, const void* pre, const void* x,
+                          long long ldx, const void* weight, long long ldw, void* grad_x,
+                          long long lddx, void* grad_weight, void* grad_bias, long long M,
+                          int N, int K, int dtype, int activation, void* workspace,
+                          long long workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -6,7 +6,7 @@ temporal head's operators that go in front of them.
 """
 from .project_layer import (PackedHeatmaps, ProcessLayerNHWC, ProjectLayer,  # noqa: F401
                             ProjectLayerWithMask)
-from .temporal import gated_recurrence  # noqa: F401
+from .temporal import fused_linear, gated_recurrence  # noqa: F401
 
 __all__ = ['ProjectLayer', 'ProjectLayerWithMask', 'ProcessLayerNHWC', 'PackedHeatmaps',
-           'gated_recurrence']
+           'fused_linear', 'gated_recurrence']

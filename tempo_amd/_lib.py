@@ -101,6 +101,12 @@ SIGNATURES = {
     'tempo_recurrence_backward': (_c_int, _strided * 3 + [_c_void_p] * 3 + _strided * 2 +
                                   [_c_void_p, _c_ll] + [_c_int] * 3 +
                                   [_c_void_p, _c_ll, _c_void_p]),
+    'tempo_linear_workspace': (_c_ll, [_c_ll] + [_c_int] * 5),
+    'tempo_linear': (_c_int, [_c_void_p, _c_ll] * 2 + [_c_void_p] + [_c_void_p, _c_ll] * 2 +
+                     [_c_void_p, _c_ll] + [_c_int] * 4 + [_c_void_p, _c_ll, _c_void_p]),
+    'tempo_linear_backward': (_c_int, [_c_void_p, _c_ll, _c_void_p] + [_c_void_p, _c_ll] * 3 +
+                              [_c_void_p] * 2 + [_c_ll] + [_c_int] * 4 +
+                              [_c_void_p, _c_ll, _c_void_p]),
 }
 
 _lib = None

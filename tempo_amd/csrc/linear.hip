@@ -1,0 +1,720 @@
+// MI355X (gfx950) kernels + C ABI of the fused linear layer and its gradients.
+//
+//   forward   z = x W^T + b          y = act(z) + r
+//   backward  dz = g * act'(z)       dx = dz W    dW = dz^T x    db = sum over rows of dz
+// x [M, K], W [N, K] (a 1x1 convolution's weight), y, r, g [M, N].
+//
+// All three products run through one tile kernel, C[i, j] = sum_k A(i, k) B(j, k), whose
+// operands lie in memory either with k adjacent (K_ADJACENT: x and W in the forward, dz in
+// dx) or with their own rows' index adjacent (ROW_ADJACENT: W in dx, both in dW).  Nothing is
+// transposed in memory: 16-bit ROW_ADJACENT tiles are turned by the LDS's transposing read
+// (ds_read_b64_tr_b16), fp32 tiles are read one k at a time, which v_mfma_f32_32x32x2_f32
+// wants anyway.
+//
+// Rounding.  Products and sums are fp32 (fp32 inputs: fp32 matrix instructions, no split or
+// shortened operands).  The epilogue is fp32 and rounds y once.  Two choices round to the
+// tensors' type in between: z is kept for the backward pass in that type, and dz is an operand
+// of two products in that type; both are half a step of a value that the products average
+// over, no more than the rounding of their outputs.  db is summed from unrounded dz.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/tempo_unproject.h"
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256;
+
+template <typename T, int V>
+struct Pack {  // element-aligned: rows of odd width start anywhere
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+
+// ---------------------------------------------------------------------------- activations
+
+enum { NONE = TEMPO_ACT_NONE, RELU = TEMPO_ACT_RELU, SILU = TEMPO_ACT_SILU,
+       GELU = TEMPO_ACT_GELU, SIGMOID = TEMPO_ACT_SIGMOID, TANH = TEMPO_ACT_TANH };
+
+__device__ __forceinline__ float fast_exp(float x) {
+  return __builtin_amdgcn_exp2f(x * 1.44269504088896341f);
+}
+
+template <bool FULL>
+__device__ __forceinline__ float sigmoid(float z) {
+  const float e = FULL ? expf(-fabsf(z)) : fast_exp(-fabsf(z));
+  const float r = FULL ? 1.f / (1.f + e) : __builtin_amdgcn_rcpf(1.f + e);
+  return z < 0.f ? e * r : (z != z ? z : r);
+}
+
+// Phi(z), the normal distribution.  16-bit results: Abramowitz & Stegun 7.1.26 for
+// erfc(|z| / sqrt 2), absolute error 1.5e-7, whose e^(-z^2 / 2) the derivative needs too.
+template <bool FULL>
+__device__ __forceinline__ float normal_cdf(float z, float* density) {
+  const float c = 0.3989422804014327f;  // 1 / sqrt(2 pi)
+  if constexpr (FULL) {
+    *density = c * expf(-0.5f * z * z);
+    return 0.5f * erfcf(-0.7071067811865476f * z);
+  } else {
+    const float x = 0.7071067811865476f * fabsf(z);
+    const float e = fast_exp(-x * x);
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float half = 0.5f * p * t * e;
+    *density = c * e;
+    return z < 0.f ? half : 1.f - half;
+  }
+}
+
+template <bool FULL>
+__device__ __forceinline__ float tanh_of(float z) {
+  if constexpr (FULL) return tanhf(z);
+  const float a = fabsf(z);
+  const float e = fast_exp(-2.f * a);
+  // next to 0 the quotient cancels: the series' error is 2/15 z^5 there
+  const float t = a < 0.03f ? fmaf(-0.33333333f * a * a, a, a)
+                            : (1.f - e) * __builtin_amdgcn_rcpf(1.f + e);
+  return copysignf(t, z);
+}
+
+template <bool FULL>
+__device__ __forceinline__ float activate(float z, int act) {
+  float density;
+  switch (act) {
+    case RELU: return z < 0.f ? 0.f : z;  // a NaN passes
+    case SILU: return z * sigmoid<FULL>(z);
+    case GELU: return z * normal_cdf<FULL>(z, &density);
+    case SIGMOID: return sigmoid<FULL>(z);
+    case TANH: return tanh_of<FULL>(z);
+    default: return z;
+  }
+}
+
+template <bool FULL>
+__device__ __forceinline__ float slope(float z, int act) {
+  float density;
+  switch (act) {
+    case RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
+    case SILU: {
+      const float s = sigmoid<FULL>(z), n = sigmoid<FULL>(-z);
+      return fmaf(z * s, n, s);
+    }
+    case GELU: {
+      const float p = normal_cdf<FULL>(z, &density);
+      return fmaf(z, density, p);
+    }
+    case SIGMOID: return sigmoid<FULL>(z) * sigmoid<FULL>(-z);
+    case TANH: {  // 1 - tanh^2 = 4 sigmoid(2z) sigmoid(-2z), which does not cancel
+      return 4.f * sigmoid<FULL>(2.f * z) * sigmoid<FULL>(-2.f * z);
+    }
+    default: return 1.f;
+  }
+}
+
+// z in the tensors' type for the backward pass: relu asks for its sign, which an fp16
+// underflow would lose
+template <typename T>
+__device__ __forceinline__ T keep_sign(float z) {
+  T r = (T)z;
+  if constexpr (sizeof(T) == 2) {
+    if (z > 0.f && (float)r == 0.f) {
+      const uint16_t least = 1;
+      __builtin_memcpy(&r, &least, 2);
+    }
+  }
+  return r;
+}
+
+// ------------------------------------------------------------------------------ tile kernel
+
+enum { K_ADJACENT = 0, ROW_ADJACENT = 1 };
+
+struct Epilogue {
+  const void *bias, *residual;  // of the output's type, or NULL
+  void *out, *pre;              // pre: z, or NULL
+  float* partial;               // not NULL: raw sums [split][I][J] instead of the above
+  long long ldr, ldo, ldp;
+  int act;
+};
+
+struct TileArgs {
+  const void *a, *b;
+  long long lda, ldb;  // elements between rows (K_ADJACENT) or between k (ROW_ADJACENT)
+  long long I, J, K;
+  uint32_t ti, tj;     // tiles
+  uint32_t split;      // parts of K, each k_part long (a multiple of the step)
+  long long k_part;
+  Epilogue e;
+};
+
+template <typename T>
+struct Mfma;
+template <>
+struct Mfma<float> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c,
+                                               0, 0, 0);
+    return c;
+  }
+};
+template <>
+struct Mfma<_Float16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<__bf16> {
+  static __device__ __forceinline__ f32x16 run(u32x4 a, u32x4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+
+// E elements at p, of which those at or beyond `left` are not in memory and count as 0
+template <typename T>
+__device__ __forceinline__ u32x4 load16(const T* p, long long left) {
+  constexpr int E = 16 / sizeof(T);
+  if (left >= E) {
+    const typename Pack<T, E>::type r = *reinterpret_cast<const typename Pack<T, E>::type*>(p);
+    return __builtin_bit_cast(u32x4, r);
+  }
+  T r[E];
+#pragma unroll
+  for (int j = 0; j < E; ++j) r[j] = j < left ? p[j] : (T)0.f;
+  u32x4 out;
+  __builtin_memcpy(&out, r, 16);
+  return out;
+}
+
+// One operand's tile in LDS: ROWS rows x 128 bytes of k.  16-byte chunks are permuted within
+// their row so that the reads below hit every bank equally:
+//   K_ADJACENT    [row][k]: chunk c of row r at c ^ (r % 8)
+//   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4);  fp32: as it is
+template <typename T, int LAYOUT, int ROWS>
+struct Tile {
+  static constexpr int E = 16 / sizeof(T);
+  static constexpr int kDepth = 128 / sizeof(T);
+  static constexpr int kLine = LAYOUT == K_ADJACENT ? 8 : ROWS / E;  // chunks per line
+  static constexpr int kBytes = ROWS * 128;
+  static constexpr int kPerThread = ROWS * 8 / kThreads;
+
+  static __device__ __forceinline__ uint32_t place(uint32_t line, uint32_t c) {
+    if constexpr (LAYOUT == K_ADJACENT)
+      return (line * 8 + (c ^ (line & 7))) * 16;
+    else if constexpr (sizeof(T) == 2)
+      return (line * kLine + (c ^ (4 * (line & 3)))) * 16;
+    else
+      return (line * kLine + c) * 16;
+  }
+
+  static __device__ __forceinline__ void fetch(const T* p, long long ld, long long row0,
+                                               long long rows, long long k0, long long k_end,
+                                               u32x4 (&r)[kPerThread]) {
+#pragma unroll
+    for (int n = 0; n < kPerThread; ++n) {
+      const uint32_t q = n * kThreads + threadIdx.x;
+      const uint32_t line = q / kLine, c = q % kLine;
+      if constexpr (LAYOUT == K_ADJACENT) {
+        const long long row = row0 + line, k = k0 + c * E;
+        r[n] = load16<T>(p + row * ld + k, row < rows ? k_end - k : 0);
+      } else {
+        const long long row = row0 + c * E, k = k0 + line;
+        r[n] = load16<T>(p + k * ld + row, k < k_end ? rows - row : 0);
+      }
+    }
+  }
+
+  static __device__ __forceinline__ void put(char* lds, const u32x4 (&r)[kPerThread]) {
+#pragma unroll
+    for (int n = 0; n < kPerThread; ++n) {
+      const uint32_t q = n * kThreads + threadIdx.x;
+      *reinterpret_cast<u32x4*>(lds + place(q / kLine, q % kLine)) = r[n];
+    }
+  }
+
+  // rows row0 .. row0 + 31 (lane % 32) x the k of step s: lanes 0..31 hold its first half,
+  // 32..63 its second
+  static __device__ __forceinline__ u32x4 fragment(const char* lds, uint32_t row0, uint32_t s,
+                                                   uint32_t lane) {
+    if constexpr (LAYOUT == K_ADJACENT) {
+      return *reinterpret_cast<const u32x4*>(lds + place(row0 + lane % 32, 2 * s + lane / 32));
+    } else if constexpr (sizeof(T) == 2) {
+      // 16 lanes read 4 lines of 16 rows; lane i of them gets row i of the 4 lines
+      typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+      const uint32_t line = 16 * s + 8 * (lane / 32) + lane % 16 / 4;
+      const uint32_t row = row0 + lane / 16 % 2 * 16 + lane % 4 * 4;
+      const uint32_t low = (row * 2) & 8;
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_i16x4*)(lds + place(line, row / 8) + low));
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_i16x4*)(lds + place(line + 4, row / 8) + low));
+      u32x4 out;
+      __builtin_memcpy(&out, &lo, 8);
+      __builtin_memcpy(reinterpret_cast<char*>(&out) + 8, &hi, 8);
+      return out;
+    } else {
+      u32x4 out;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        out[j] = *reinterpret_cast<const uint32_t*>(
+            lds + ((8 * s + 4 * (lane / 32) + j) * ROWS + row0 + lane % 32) * 4);
+      return out;
+    }
+  }
+};
+
+// Tiles go to the 8 XCDs (workgroups are dealt to them in turn) in contiguous runs, and within
+// a run 8 tile rows at a time, so that one L2 sees few different rows of both operands.
+__device__ __forceinline__ void tile_of(uint32_t id, uint32_t ti, uint32_t tj, uint32_t* i,
+                                        uint32_t* j) {
+  const uint32_t n = ti * tj, per = n / 8, rest = n % 8, x = id % 8;
+  const uint32_t t = x * per + min(x, rest) + id / 8;
+  const uint32_t group = t / (8 * tj), first = group * 8, high = min(8u, ti - first);
+  const uint32_t in = t - group * 8 * tj;
+  *i = first + in % high;
+  *j = in / high;
+}
+
+template <typename T>
+__device__ __forceinline__ void finish(const Epilogue& e, long long i, long long j, int n,
+                                       f32x4 acc) {
+  constexpr bool FULL = sizeof(T) == 4;
+  typedef typename Pack<T, 4>::type V4;
+  float z[4], y[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) z[q] = acc[q];
+  if (n == 4) {
+    if (e.bias) {
+      const V4 b = *reinterpret_cast<const V4*>((const T*)e.bias + j);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) z[q] += (float)b[q];
+    }
+    if (e.pre) {
+      V4 p;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) p[q] = keep_sign<T>(z[q]);
+      *reinterpret_cast<V4*>((T*)e.pre + i * e.ldp + j) = p;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) y[q] = activate<FULL>(z[q], e.act);
+    if (e.residual) {
+      const V4 r = *reinterpret_cast<const V4*>((const T*)e.residual + i * e.ldr + j);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) y[q] += (float)r[q];
+    }
+    V4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = (T)y[q];
+    *reinterpret_cast<V4*>((T*)e.out + i * e.ldo + j) = o;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (q < n) {
+        if (e.bias) z[q] += (float)((const T*)e.bias)[j + q];
+        if (e.pre) ((T*)e.pre)[i * e.ldp + j + q] = keep_sign<T>(z[q]);
+        float v = activate<FULL>(z[q], e.act);
+        if (e.residual) v += (float)((const T*)e.residual)[i * e.ldr + j + q];
+        ((T*)e.out)[i * e.ldo + j + q] = (T)v;
+      }
+    }
+  }
+}
+
+// 128 x 128 of C per workgroup, 4 waves of 64 x 64; loads of the next 128 bytes of k fly under
+// the products of the present ones.
+template <typename T, int AL, int BL>
+__global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
+  typedef Tile<T, AL, 128> TA;
+  typedef Tile<T, BL, 128> TB;
+  __shared__ __attribute__((aligned(16))) char lds[2][TA::kBytes + TB::kBytes];
+  uint32_t i_tile, j_tile;
+  tile_of(blockIdx.x, a.ti, a.tj, &i_tile, &j_tile);
+  const long long i0 = (long long)i_tile * 128, j0 = (long long)j_tile * 128;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t wi = wave / 2 * 64, wj = wave % 2 * 64;
+  const long long k_begin = blockIdx.y * a.k_part;
+  const long long k_end = min(a.K, k_begin + a.k_part);
+  const T *pa = (const T*)a.a, *pb = (const T*)a.b;
+
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+
+  u32x4 ra[TA::kPerThread], rb[TB::kPerThread];
+  TA::fetch(pa, a.lda, i0, a.I, k_begin, k_end, ra);
+  TB::fetch(pb, a.ldb, j0, a.J, k_begin, k_end, rb);
+  TA::put(lds[0], ra);
+  TB::put(lds[0] + TA::kBytes, rb);
+  __syncthreads();
+  int now = 0;
+  for (long long k = k_begin; k < k_end; k += TA::kDepth, now ^= 1) {
+    const bool more = k + TA::kDepth < k_end;
+    if (more) {
+      TA::fetch(pa, a.lda, i0, a.I, k + TA::kDepth, k_end, ra);
+      TB::fetch(pb, a.ldb, j0, a.J, k + TA::kDepth, k_end, rb);
+    }
+    const char* la = lds[now];
+    const char* lb = la + TA::kBytes;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u32x4 fa[2], fb[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) fa[x] = TA::fragment(la, wi + 32 * x, s, lane);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) fb[y] = TB::fragment(lb, wj + 32 * y, s, lane);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y)  // C^T: a lane holds 4 neighbouring j of one i
+          acc[x][y] = Mfma<T>::run(fb[y], fa[x], acc[x][y]);
+    }
+    if (more) {
+      TA::put(lds[now ^ 1], ra);
+      TB::put(lds[now ^ 1] + TA::kBytes, rb);
+    }
+    __syncthreads();
+  }
+
+  // The tile's sums pass through LDS (64 KB, the operands are done with): a wave holds columns
+  // of rows, memory wants rows.  16-byte chunk c of row i lies at c ^ (i % 32).
+  char* lc = lds[0];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t i = wi + 32 * x + lane % 32, c = (wj + 32 * y + 8 * g) / 4 + lane / 32;
+        const f32x4 v = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2],
+                         acc[x][y][4 * g + 3]};
+        *reinterpret_cast<f32x4*>(lc + (i * 32 + (c ^ (i & 31))) * 16) = v;
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t c = threadIdx.x % 32;
+  const long long j = j0 + c * 4;
+  if (j >= a.J) return;
+  const int n = (int)min(4ll, a.J - j);
+  const uint32_t high = (uint32_t)min(128ll, a.I - i0);
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x / 32; i < high; i += kThreads / 32) {
+    const f32x4 v = *reinterpret_cast<const f32x4*>(lc + (i * 32 + (c ^ (i & 31))) * 16);
+    if (a.e.partial) {
+      float* p = a.e.partial + ((long long)blockIdx.y * a.I + i0 + i) * a.J + j;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < n) p[q] = v[q];
+    } else {
+      finish<T>(a.e, i0 + i, j, n, v);
+    }
+  }
+}
+
+// The parts of a K that was split, in order, then the epilogue.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, uint32_t split,
+                                                        long long I, long long J, Epilogue e) {
+  const long long quads = (J + 3) / 4;
+  const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
+  if (id >= I * quads) return;
+  const long long i = id / quads, j = (id - i * quads) * 4;
+  const int n = (int)min(4ll, J - j);
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  const float* p = partial + i * J + j;
+  for (uint32_t s = 0; s < split; ++s, p += I * J) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < n) sum[q] += p[q];
+  }
+  finish<T>(e, i, j, n, sum);
+}
+
+// --------------------------------------------------------------- gradient of z, bias gradient
+
+constexpr int kRowsPerBlock = 512;
+
+// dz = g * act'(z) in the tensors' type (unless dz is NULL) and the sums of the unrounded
+// values over the workgroup's rows.  A thread owns 4 columns, 8 threads side by side.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long ldg, const T* pre,
+                                                          T* dz, float* sums, long long M, int N,
+                                                          int act) {
+  constexpr bool FULL = sizeof(T) == 4;
+  __shared__ float s_sum[32][33];
+  const int j = blockIdx.y * 32 + threadIdx.x % 8 * 4;
+  const int r = threadIdx.x / 8;
+  const long long first = (long long)blockIdx.x * kRowsPerBlock;
+  const long long stop = min(M, first + kRowsPerBlock);
+  const int n = max(0, min(4, N - j));
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  for (long long i = first + r; i < stop; i += 32) {
+    if (n == 4) {
+      typedef typename Pack<T, 4>::type V4;
+      const V4 gv = *reinterpret_cast<const V4*>(g + i * ldg + j);
+      V4 zv = gv, out;
+      if (pre) zv = *reinterpret_cast<const V4*>(pre + i * N + j);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float d = (float)gv[q] * slope<FULL>((float)zv[q], act);
+        sum[q] += d;
+        out[q] = (T)d;
+      }
+      if (dz) *reinterpret_cast<V4*>(dz + i * N + j) = out;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (q < n) {
+          const float z = pre ? (float)pre[i * N + j + q] : 0.f;
+          const float d = (float)g[i * ldg + j + q] * slope<FULL>(z, act);
+          sum[q] += d;
+          if (dz) dz[i * N + j + q] = (T)d;
+        }
+      }
+    }
+  }
+  if (!sums) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) s_sum[threadIdx.x % 8 * 4 + q][r] = sum[q];
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    float total = 0.f;
+    for (int k = 0; k < 32; ++k) total += s_sum[threadIdx.x][k];
+    const int col = blockIdx.y * 32 + threadIdx.x;
+    if (col < N) sums[(long long)blockIdx.x * N + col] = total;
+  }
+}
+
+// bias gradient from the row blocks' sums: a workgroup owns 8 columns
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_bias_kernel(const float* sums, long long blocks,
+                                                             int N, T* out) {
+  __shared__ float s_sum[32][9];
+  const int col = blockIdx.x * 8 + threadIdx.x % 8, r = threadIdx.x / 8;
+  float sum = 0.f;
+  if (col < N)
+    for (long long b = r; b < blocks; b += 32) sum += sums[b * N + col];
+  s_sum[r][threadIdx.x % 8] = sum;
+  __syncthreads();
+  if (threadIdx.x < 8 && col < N) {
+    float total = 0.f;
+    for (int k = 0; k < 32; ++k) total += s_sum[k][threadIdx.x];
+    out[col] = (T)total;
+  }
+}
+
+// ------------------------------------------------------------------------------------- host
+
+constexpr int kUnits = 256;  // compute units to fill
+
+struct Product {
+  uint32_t ti, tj, split;
+  long long k_part;
+  long long bytes(long long I, long long J) const {
+    return split > 1 ? (long long)split * I * J * 4 : 0;
+  }
+};
+
+// K is split where the tiles alone leave compute units idle, into parts of at least four
+// steps (512 bytes of k).
+bool plan_product(long long I, long long J, long long K, int dtype, Product* p) {
+  const long long ti = (I + 127) / 128, tj = (J + 127) / 128;
+  if (ti > 0x3fffffff / tj) return false;
+  p->ti = (uint32_t)ti;
+  p->tj = (uint32_t)tj;
+  const long long depth = dtype == TEMPO_DTYPE_F32 ? 32 : 64;
+  const long long steps = (K + depth - 1) / depth;
+  long long split = 2 * kUnits / (ti * tj);
+  if (split > steps / 4) split = steps / 4;
+  if (split < 1) split = 1;
+  const long long part = (steps + split - 1) / split;
+  p->k_part = part * depth;
+  p->split = (uint32_t)((steps + part - 1) / part);
+  return p->split <= 65535;
+}
+
+template <typename T, int AL, int BL>
+int run_product(const Product& p, const void* a, long long lda, const void* b, long long ldb,
+                long long I, long long J, long long K, const Epilogue& e, float* scratch,
+                hipStream_t stream) {
+  TileArgs t = {};
+  t.a = a; t.b = b; t.lda = lda; t.ldb = ldb; t.I = I; t.J = J; t.K = K;
+  t.ti = p.ti; t.tj = p.tj; t.split = p.split; t.k_part = p.k_part;
+  t.e = e;
+  t.e.partial = p.split > 1 ? scratch : nullptr;
+  hipLaunchKernelGGL((tile_kernel<T, AL, BL>), dim3(p.ti * p.tj, p.split), dim3(kThreads), 0,
+                     stream, t);
+  if (p.split > 1) {
+    const long long quads = I * ((J + 3) / 4);
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((quads + kThreads - 1) / kThreads)),
+                       dim3(kThreads), 0, stream, scratch, p.split, I, J, e);
+  }
+  return (int)hipGetLastError();
+}
+
+struct BackwardPlan {
+  Product dx, dw;
+  long long dz_bytes, sum_bytes, scratch_bytes;
+  long long total() const { return dz_bytes + sum_bytes + scratch_bytes; }
+};
+
+long long up16(long long n) { return (n + 15) / 16 * 16; }
+
+bool plan_backward(long long M, int N, int K, int dtype, int act, BackwardPlan* p) {
+  if (!plan_product(M, K, N, dtype, &p->dx) || !plan_product(N, K, M, dtype, &p->dw))
+    return false;
+  p->dz_bytes = act == NONE ? 0 : up16(M * N * (dtype == TEMPO_DTYPE_F32 ? 4 : 2));
+  p->sum_bytes = up16((M + kRowsPerBlock - 1) / kRowsPerBlock * N * 4);
+  const long long x = p->dx.bytes(M, K), w = p->dw.bytes(N, K);
+  p->scratch_bytes = up16(x > w ? x : w);
+  return true;
+}
+
+int check_sizes(long long M, int N, int K, int dtype, int act) {
+  if (M <= 0 || N <= 0 || K <= 0) return TEMPO_E_DIM;
+  if (dtype != TEMPO_DTYPE_F32 && dtype != TEMPO_DTYPE_F16 && dtype != TEMPO_DTYPE_BF16)
+    return TEMPO_E_ARG;
+  if (act < NONE || act > TANH) return TEMPO_E_ARG;
+  if (M > 0x7fffffffLL || N > (1 << 20) || K > (1 << 20)) return TEMPO_E_SIZE;
+  return TEMPO_OK;
+}
+
+bool misaligned(const void* p, int dtype) {
+  return ((uintptr_t)p & (dtype == TEMPO_DTYPE_F32 ? 3 : 1)) != 0;
+}
+
+template <typename T>
+int forward_for(const Product& p, const void* x, long long ldx, const void* w, long long ldw,
+                const Epilogue& e, long long M, int N, int K, float* scratch,
+                hipStream_t stream) {
+  return run_product<T, K_ADJACENT, K_ADJACENT>(p, x, ldx, w, ldw, M, N, K, e, scratch, stream);
+}
+
+template <typename T>
+int backward_for(const BackwardPlan& p, const void* g, long long ldg, const void* pre,
+                 const void* x, long long ldx, const void* w, long long ldw, void* dx,
+                 long long lddx, void* dw, void* db, long long M, int N, int K, int act,
+                 char* ws, hipStream_t stream) {
+  T* dz = act == NONE ? nullptr : (T*)ws;
+  float* sums = db ? (float*)(ws + p.dz_bytes) : nullptr;
+  float* scratch = (float*)(ws + p.dz_bytes + p.sum_bytes);
+  const long long blocks = (M + kRowsPerBlock - 1) / kRowsPerBlock;
+  if (dz || db) {
+    hipLaunchKernelGGL((grad_z_kernel<T>), dim3((unsigned)blocks, (N + 31) / 32), dim3(kThreads),
+                       0, stream, (const T*)g, ldg, (const T*)pre, dz, sums, M, N, act);
+    if (db)
+      hipLaunchKernelGGL((grad_bias_kernel<T>), dim3((N + 7) / 8), dim3(kThreads), 0, stream,
+                         sums, blocks, N, (T*)db);
+  }
+  const void* z = dz ? (const void*)dz : g;
+  const long long ldz = dz ? N : ldg;
+  Epilogue e = {};
+  int rc = (int)hipGetLastError();
+  if (rc == 0 && dx) {
+    e.out = dx; e.ldo = lddx;
+    rc = run_product<T, K_ADJACENT, ROW_ADJACENT>(p.dx, z, ldz, w, ldw, M, K, N, e, scratch,
+                                                  stream);
+  }
+  if (rc == 0 && dw) {
+    e.out = dw; e.ldo = K;
+    rc = run_product<T, ROW_ADJACENT, ROW_ADJACENT>(p.dw, z, ldz, x, ldx, N, K, M, e, scratch,
+                                                    stream);
+  }
+  return rc;
+}
+
+}  // namespace
+
+extern "C" {
+
+long long tempo_linear_workspace(long long M, int N, int K, int dtype, int activation,
+                                 int backward) {
+  const int rc = check_sizes(M, N, K, dtype, activation);
+  if (rc != TEMPO_OK) return rc;
+  if (backward) {
+    BackwardPlan p;
+    return plan_backward(M, N, K, dtype, activation, &p) ? p.total() : TEMPO_E_SIZE;
+  }
+  Product p;
+  return plan_product(M, N, K, dtype, &p) ? p.bytes(M, N) : TEMPO_E_SIZE;
+}
+
+int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw,
+                 const void* bias, const void* residual, long long ldr, void* y, long long ldy,
+                 void* pre, long long M, int N, int K, int dtype, int activation,
+                 void* workspace, long long workspace_bytes, void* stream) {
+  if (!x || !weight || !y) return TEMPO_E_NULL;
+  const int rc = check_sizes(M, N, K, dtype, activation);
+  if (rc != TEMPO_OK) return rc;
+  Product p;
+  if (!plan_product(M, N, K, dtype, &p)) return TEMPO_E_SIZE;
+  if (ldx < 0 || ldw < 0 || ldr < 0 || (M > 1 && ldy < N)) return TEMPO_E_ARG;
+  if (misaligned(x, dtype) || misaligned(weight, dtype) || misaligned(y, dtype) ||
+      misaligned(bias, dtype) || misaligned(residual, dtype) || misaligned(pre, dtype))
+    return TEMPO_E_ARG;
+  const long long need = p.bytes(M, N);
+  if (need > 0 && !workspace) return TEMPO_E_NULL;
+  if (need > workspace_bytes) return TEMPO_E_SIZE;
+  if ((uintptr_t)workspace & 15) return TEMPO_E_ARG;
+  Epilogue e = {};
+  e.bias = bias; e.residual = residual; e.out = y; e.pre = pre;
+  e.ldr = ldr; e.ldo = ldy; e.ldp = N; e.act = activation;
+  float* scratch = (float*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == TEMPO_DTYPE_F32)
+    return forward_for<float>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
+  if (dtype == TEMPO_DTYPE_F16)
+    return forward_for<_Float16>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
+  return forward_for<__bf16>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
+}
+
+int tempo_linear_backward(const void* grad_y, long long ldg, const void* pre, const void* x,
+                          long long ldx, const void* weight, long long ldw, void* grad_x,
+                          long long lddx, void* grad_weight, void* grad_bias, long long M, int N,
+                          int K, int dtype, int activation, void* workspace,
+                          long long workspace_bytes, void* stream) {
+  if (!grad_y || (grad_x && !weight) || (grad_weight && !x)) return TEMPO_E_NULL;
+  const int rc = check_sizes(M, N, K, dtype, activation);
+  if (rc != TEMPO_OK) return rc;
+  if (activation != NONE && !pre) return TEMPO_E_NULL;
+  BackwardPlan p;
+  if (!plan_backward(M, N, K, dtype, activation, &p)) return TEMPO_E_SIZE;
+  if (ldg < 0 || ldx < 0 || ldw < 0 || (grad_x && M > 1 && lddx < K)) return TEMPO_E_ARG;
+  if (misaligned(grad_y, dtype) || misaligned(pre, dtype) || misaligned(x, dtype) ||
+      misaligned(weight, dtype) || misaligned(grad_x, dtype) || misaligned(grad_weight, dtype) ||
+      misaligned(grad_bias, dtype))
+    return TEMPO_E_ARG;
+  if (!workspace) return TEMPO_E_NULL;
+  if (p.total() > workspace_bytes) return TEMPO_E_SIZE;
+  if ((uintptr_t)workspace & 15) return TEMPO_E_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  const void* z = activation == NONE ? nullptr : pre;
+  if (dtype == TEMPO_DTYPE_F32)
+    return backward_for<float>(p, grad_y, ldg, z, x, ldx, weight, ldw, grad_x, lddx, grad_weight,
+                               grad_bias, M, N, K, activation, ws, s);
+  if (dtype == TEMPO_DTYPE_F16)
+    return backward_for<_Float16>(p, grad_y, ldg, z, x, ldx, weight, ldw, grad_x, lddx,
+                                  grad_weight, grad_bias, M, N, K, activation, ws, s);
+  return backward_for<__bf16>(p, grad_y, ldg, z, x, ldx, weight, ldw, grad_x, lddx, grad_weight,
+                              grad_bias, M, N, K, activation, ws, s);
+}
+
+}  // extern "C"

@@ -1403,3 +1403,118 @@ def recurrence_backward(grad_h, grad_last, gate, value=None, state=None, ckpt=No
                 B, T, D, code, _ptr(ws), need, _stream_ptr(dev))
         _lib.check(rc, 'tempo_recurrence_backward')
     return dpacked, None if both else dvalue, dstate
+
+
+# --------------------------------------------------------------------------
+# temporal head: fused linear layer
+# --------------------------------------------------------------------------
+
+ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2, 'gelu': 3, 'sigmoid': 4, 'tanh': 5}  # TEMPO_ACT_*
+
+
+def _activation(name):
+    if name not in ACTIVATIONS:
+        raise ValueError(f'activation: {name!r}, expected one of {", ".join(ACTIVATIONS)}')
+    return ACTIVATIONS[name]
+
+
+def _rows(t, name, dtype=None, device=None):
+    """``[..., C]`` as ``[rows, C]`` without a copy: channels adjacent, one distance between
+    rows."""
+    if isinstance(t, torch.Tensor) and t.dim() == 0:
+        raise ValueError(f'{name}: no channels')
+    _float_tensor(t, name, t.dim() if isinstance(t, torch.Tensor) else 0, dtype, device)
+    try:
+        return t.view(t.numel() // max(t.shape[-1], 1), t.shape[-1])
+    except RuntimeError:
+        raise ValueError(f'{name}: its rows must lie at one distance from each other '
+                         f'(shape {tuple(t.shape)}, strides {t.stride()})') from None
+
+
+def _linear_operands(x, weight, bias):
+    rows = _rows(x, 'x')
+    dtype, dev = x.dtype, x.device
+    _float_tensor(weight, 'weight', 2, dtype, dev)
+    N, K = (int(n) for n in weight.shape)
+    if int(rows.shape[1]) != K:
+        raise ValueError(f'weight: expected [N,{int(rows.shape[1])}], got {tuple(weight.shape)}')
+    if N == 0 or K == 0:
+        raise ValueError('weight: no channels')
+    if bias is not None:
+        _float_tensor(bias, 'bias', 1, dtype, dev)
+        if int(bias.shape[0]) != N:
+            raise ValueError(f'bias: expected [{N}], got {tuple(bias.shape)}')
+    return rows, int(rows.shape[0]), N, K
+
+
+def linear_forward(x, weight, bias=None, residual=None, activation='none', out=None,
+                   want_pre=False):
+    """``act(x W^T + bias) + residual`` -> ``(y, pre)``; arguments as
+    :func:`tempo_amd.fused_linear` with a 2-D weight.  ``pre``: the values before the activation
+    as :func:`linear_backward` needs them (None unless ``want_pre`` and there is one)."""
+    lib = _lib.load()
+    _no_grad_path('linear_forward', x, weight, bias, residual)
+    act = _activation(activation)
+    rows, M, N, K = _linear_operands(x, weight, bias)
+    dev, code = x.device, FLOAT_DTYPES[x.dtype]
+    shape = tuple(x.shape[:-1]) + (N,)
+    res = None
+    if residual is not None:
+        if not isinstance(residual, torch.Tensor) or tuple(residual.shape) != shape:
+            raise ValueError(f'residual: expected {list(shape)}, got '
+                             f'{list(getattr(residual, "shape", []))}')
+        res = _rows(residual, 'residual', x.dtype, dev)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+    elif tuple(out.shape) != shape:
+        raise ValueError(f'out: expected {list(shape)}, got {list(out.shape)}')
+    dst = _rows(out, 'out', x.dtype, dev)
+    if M > 1 and dst.stride(0) < N:
+        raise ValueError('out: its rows overlap')
+    pre = torch.empty(M, N, dtype=x.dtype, device=dev) if want_pre and act else None
+    if M == 0:
+        return out, pre
+    with torch.cuda.device(dev):
+        need = lib.tempo_linear_workspace(M, N, K, code, act, 0)
+        ws = _workspace(need, 'tempo_linear_workspace', dev)
+        rc = lib.tempo_linear(_ptr(rows), rows.stride(0), _ptr(weight), weight.stride(0),
+                              _ptr(bias), _ptr(res), 0 if res is None else res.stride(0),
+                              _ptr(dst), dst.stride(0), _ptr(pre), M, N, K, code, act, _ptr(ws),
+                              need, _stream_ptr(dev))
+    _lib.check(rc, 'tempo_linear')
+    return out, pre
+
+
+def linear_backward(grad_y, x, weight, pre=None, activation='none', want=(True, True, True)):
+    """Gradients of :func:`linear_forward` with respect to x, weight and bias, each None where
+    ``want`` says so; the residual's is ``grad_y`` itself."""
+    lib = _lib.load()
+    act = _activation(activation)
+    rows, M, N, K = _linear_operands(x, weight, None)
+    dev, code = x.device, FLOAT_DTYPES[x.dtype]
+    if tuple(grad_y.shape) != tuple(x.shape[:-1]) + (N,):
+        raise ValueError(f'grad_y: expected {list(x.shape[:-1]) + [N]}, got '
+                         f'{list(grad_y.shape)}')
+    try:
+        g = _rows(grad_y, 'grad_y', x.dtype, dev)
+    except ValueError:  # e.g. the gradient of a sum: no memory of its own
+        g = _rows(grad_y.contiguous(), 'grad_y', x.dtype, dev)
+    if act and M:
+        _need(pre, x.dtype, 'pre', dev)
+        if tuple(pre.shape) != (M, N):
+            raise ValueError(f'pre: expected [{M},{N}], got {tuple(pre.shape)}')
+    make = torch.empty if M else torch.zeros
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
+    dw = make(N, K, dtype=x.dtype, device=dev) if want[1] else None
+    db = make(N, dtype=x.dtype, device=dev) if want[2] else None
+    if M == 0 or not any(want):
+        return dx, dw, db
+    with torch.cuda.device(dev):
+        need = lib.tempo_linear_workspace(M, N, K, code, act, 1)
+        ws = _workspace(need, 'tempo_linear_workspace', dev)
+        rc = lib.tempo_linear_backward(_ptr(g), g.stride(0), _ptr(pre), _ptr(rows),
+                                       rows.stride(0), _ptr(weight), weight.stride(0), _ptr(dx),
+                                       K, _ptr(dw), _ptr(db), M, N, K, code, act, _ptr(ws),
+                                       need, _stream_ptr(dev))
+    _lib.check(rc, 'tempo_linear_backward')
+    return dx, dw, db

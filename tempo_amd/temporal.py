@@ -70,3 +70,48 @@ def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state
         return _GatedRecurrence.apply(gate, value, state, lengths)
     h, last, _ = ops.recurrence_forward(gate, value, state, lengths, out, state_out)
     return h, last
+
+
+class _FusedLinear(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        y, pre = ops.linear_forward(x, weight, bias, residual, activation, want_pre=True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.linear_backward(grad_y, x, weight, pre, ctx.activation, need[:3])
+        return dx, dw, db, grad_y if need[3] else None, None
+
+
+def fused_linear(x, weight, bias=None, residual=None, activation='none', out=None):
+    """``act(x W^T + bias) + residual`` in one pass over memory: a 1x1 convolution of
+    channel-last maps with its epilogue.
+
+    ``x``: ``[..., K]`` in fp32, fp16 or bf16, channels adjacent and rows at one distance from
+    each other (a ``torch.channels_last`` map is ``map.permute(0, 2, 3, 1)``); ``weight``
+    ``[N,K]`` or a convolution's ``[N,K,1,1]``; ``bias`` ``[N]``; ``residual`` ``[..., N]``, all
+    of x's type.  ``activation``: none, relu, silu, gelu (with the normal distribution itself),
+    sigmoid or tanh.  Returns ``[..., N]``.
+
+    Sums are fp32, the result is rounded once; fp32 inputs are multiplied in fp32.
+    Differentiable once, with respect to every tensor; for the backward pass the value in front
+    of the activation is kept in x's type, as a layer's output would be.  ``out`` (not under
+    autograd): where to write the result.
+
+    To capture a training step into a graph, drop eager results of the same leaves first: torch
+    itself ends the process when a captured backward meets their gradient accumulators."""
+    if isinstance(weight, torch.Tensor) and weight.dim() == 4 and weight.shape[2:] == (1, 1):
+        weight = weight.flatten(1)
+    if _records(x, weight, bias, residual):
+        if out is not None:
+            raise NotImplementedError('fused_linear: out is for calls without gradients '
+                                      '(torch.no_grad() or detached tensors)')
+        return _FusedLinear.apply(x, weight, bias, residual, activation)
+    return ops.linear_forward(x, weight, bias, residual, activation, out)[0]

@@ -92,3 +92,87 @@ def check(got, ref, tol, what):
         f'{what}: {int((over > 0).sum())} of {over.numel()} beyond the tolerance, worst '
         f'{float((got - ref).abs().max()):.3e} at tolerance '
         f'{float(tol.flatten()[over.flatten().argmax()]):.3e}')
+
+
+# ------------------------------------------------------------------------- fused linear layer
+
+_ACT = {
+    'none': (lambda z: z, lambda z: torch.ones_like(z)),
+    'relu': (lambda z: z.clamp(min=0), lambda z: (z > 0).double()),
+    'silu': (lambda z: z * z.sigmoid(), lambda z: z.sigmoid() * (1 + z * (-z).sigmoid())),
+    'gelu': (lambda z: z * torch.special.ndtr(z),
+             lambda z: torch.special.ndtr(z) + z * torch.exp(-z * z / 2) * 0.3989422804014327),
+    'sigmoid': (torch.sigmoid, lambda z: z.sigmoid() * (-z).sigmoid()),
+    'tanh': (torch.tanh, lambda z: 1 - torch.tanh(z) ** 2),
+}
+# largest |act'|, |act''|
+_STEEP = {'none': (1.0, 0.0), 'relu': (1.0, 0.0), 'silu': (1.1, 0.5), 'gelu': (1.13, 0.8),
+          'sigmoid': (0.25, 0.1), 'tanh': (1.0, 0.77)}
+
+
+def linear(x, weight, bias=None, residual=None, activation='none', grad=None):
+    """dict of y (and dx, dweight, dbias) in fp64 on the CPU with tolerances for kernels that
+    return ``x.dtype``.
+
+    Let u = 2^-24.  A sum of n products in fp32, in any order, errs by at most
+    (n + 1) u sum |a b|; the matrix units may drop what lies under the last bit of an operand's
+    alignment, another n u.  z errs by dz0 = 2 (K + 2) u (|x| |W|^T + |b|), the activation by its
+    steepness times that plus a few u of its own (16 bits: 2^-19 of its value, erfc's 2^-22
+    absolute times |z|).  Backwards: z is kept to half a step, so act' errs by its steepness
+    times (dz0 + half a step of z); dz is rounded by half a step; the products add their
+    n + 1 terms' error and one rounding."""
+    dtype = x.dtype
+    X, W = x.double().cpu(), weight.double().cpu()
+    shape = X.shape
+    X = X.reshape(-1, shape[-1])
+    M, K = X.shape
+    N = W.shape[0]
+    u = 2.0 ** -24
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    act, slope = _ACT[activation]
+    steep, bend = _STEEP[activation]
+    z = X @ W.t()
+    z_err = X.abs() @ W.abs().t()
+    if bias is not None:
+        z = z + bias.double().cpu()
+        z_err = z_err + bias.double().cpu().abs()
+    z_err = 2 * (K + 2) * u * z_err
+    own = (2.0 ** -21 if dtype == torch.float32 else 2.0 ** -19)
+    a = act(z)
+    y = a
+    y_err = steep * z_err
+    if activation != 'none' and activation != 'relu':
+        y_err = y_err + own * a.abs() + 2.0 ** -22 * (z.abs() + 1)
+    if residual is not None:
+        res = residual.double().cpu().reshape(M, N)
+        y = y + res
+        y_err = y_err + 2 * u * (a.abs() + res.abs())
+    r = {'y': y.reshape(shape[:-1] + (N,))}
+    r['y_tol'] = (y_err + rounding(y, dtype)).reshape(r['y'].shape)
+    if grad is None:
+        return r
+    g = grad.double().cpu().reshape(M, N)
+    s = slope(z)
+    dz = g * s
+    s_err = bend * (z_err + half * z.abs()) + own * (1 + z.abs()) * (activation not in
+                                                                     ('none', 'relu'))
+    if activation == 'relu':
+        # the sign of a z within its error of 0 may be either
+        s_err = (z.abs() <= z_err).double()
+    dz_err = g.abs() * s_err + 4 * u * dz.abs()
+    dz_op = dz_err if activation == 'none' and half else \
+        dz_err + (rounding(dz, dtype) if half else 0)
+    if activation == 'none':
+        dz_op = torch.zeros_like(dz)
+    big = dz.abs() + dz_op
+    r['dx'] = (dz @ W).reshape(shape)
+    r['dx_tol'] = (dz_op @ W.abs() + 2 * (N + 2) * u * (big @ W.abs())).reshape(shape) + \
+        rounding(r['dx'], dtype)
+    r['dweight'] = dz.t() @ X
+    # parts of a split sum are joined in fp32, too: twice the terms' bound covers that
+    r['dweight_tol'] = dz_op.t() @ X.abs() + 2 * (M + 2) * u * (big.t() @ X.abs()) + \
+        rounding(r['dweight'], dtype)
+    r['dbias'] = dz.sum(0)
+    r['dbias_tol'] = dz_err.sum(0) + 2 * (M + 2) * u * dz.abs().sum(0) + \
+        rounding(r['dbias'], dtype)
+    return r

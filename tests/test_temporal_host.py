@@ -61,3 +61,54 @@ def test_no_cpu_path():
     x = torch.zeros(2, 3, 8)
     with pytest.raises(TypeError):
         tempo_amd.gated_recurrence(x, x)
+    with pytest.raises(TypeError):
+        tempo_amd.fused_linear(x, torch.zeros(4, 8))
+
+
+def test_linear_entry_points_reject_bad_arguments():
+    lib = _lib.load()
+
+    def forward(**kw):
+        g = kw.get
+        return lib.tempo_linear(
+            g('x', ONE), g('ldx', 64), g('weight', ONE), g('ldw', 64), g('bias', None),
+            g('residual', None), g('ldr', 16), g('y', ONE), g('ldy', 16), g('pre', None),
+            g('M', 4), g('N', 16), g('K', 64), g('dtype', 0), g('act', 0), g('ws', ONE),
+            g('bytes', 1 << 40), None)
+
+    def backward(**kw):
+        g = kw.get
+        return lib.tempo_linear_backward(
+            g('grad', ONE), g('ldg', 16), g('pre', None), g('x', ONE), g('ldx', 64),
+            g('weight', ONE), g('ldw', 64), g('dx', ONE), g('lddx', 64), g('dw', ONE),
+            g('db', ONE), g('M', 4), g('N', 16), g('K', 64), g('dtype', 0), g('act', 0),
+            g('ws', ONE), g('bytes', 1 << 40), None)
+
+    for name in ('x', 'weight', 'y'):
+        assert forward(**{name: None}) == -1
+    for name in ('x', 'weight', 'grad', 'ws'):
+        assert backward(**{name: None}) == -1
+    assert backward(act=1) == -1  # its z is missing
+    for call in (forward, backward):
+        assert call(M=0) == -2 and call(N=0) == -2 and call(K=-1) == -2
+        assert call(dtype=3) == -5 and call(act=6) == -5 and call(act=-1) == -5
+        assert call(x=P(18)) == -5 and call(weight=P(17), dtype=2) == -5
+        assert call(M=1 << 32) == -4 and call(N=1 << 21) == -4 and call(K=1 << 21) == -4
+        assert call(ldx=-1) == -5 and call(ldw=-1) == -5
+        assert call(ws=P(24), K=65536, bytes=1 << 40) == -5
+        assert call(K=65536, bytes=8, lddx=65536) == -4
+    assert forward(K=65536, ws=None) == -1
+    assert forward(ldy=15) == -5 and backward(lddx=63) == -5 and backward(ldg=-1) == -5
+    for name in ('y', 'bias', 'residual', 'pre'):
+        assert forward(**{name: P(18)}) == -5
+    for name in ('grad', 'dx', 'dw', 'db'):
+        assert backward(**{name: P(18)}) == -5
+    assert backward(pre=P(18), act=1) == -5
+
+
+def test_linear_workspace():
+    ws = _lib.load().tempo_linear_workspace
+    assert ws(0, 1, 1, 0, 0, 0) == -2 and ws(1, 1, 1, 7, 0, 0) == -5
+    assert ws(1, 1, 1, 0, 9, 0) == -5 and ws(1, 1 << 21, 1, 0, 0, 0) == -4
+    assert ws(16384, 4096, 4096, 2, 0, 0) == 0  # tiles enough: the sum is not split
+    assert ws(8192, 4096, 1024, 2, 3, 1) >= 8192 * 4096 * 2  # dz
