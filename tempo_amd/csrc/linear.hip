@@ -428,6 +428,198 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
   }
 }
 
+// ---------------------------------------------------- tile kernel on aligned operands
+//
+// The same product where every 16-byte chunk of both operands is aligned and wholly inside or
+// outside of its row: tiles go from memory straight to LDS (buffer_load ... lds), so no
+// register holds data in flight and a workgroup can be 256 x 256, which halves what each
+// product reads from LDS.  Chunks outside an operand carry an offset beyond the buffer's
+// range, for which the hardware writes zeros.  A chunk's place in LDS follows from its lane
+// (base + 16 lane), hence the lane picks the chunk that belongs to its place.
+
+constexpr uint32_t kOutside = 0x80000000u;
+
+__device__ __forceinline__ u32x4 buffer_of(const void* p, uint32_t bytes) {
+  const uint64_t at = (uint64_t)p;
+  u32x4 r = {(uint32_t)at, (uint32_t)(at >> 32), bytes, 0x00020000u};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) r[q] = __builtin_amdgcn_readfirstlane(r[q]);
+  return r;
+}
+
+// 64 chunks to LDS bytes lds .. lds + 1023; the caller waits (vmcnt) before anyone reads them
+__device__ __forceinline__ void chunks_to_lds(uint32_t lds, uint32_t offset, u32x4 buffer,
+                                              uint32_t scalar_offset) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
+      "v"(offset), "s"(buffer), "s"(scalar_offset)
+      : "memory", "m0");
+}
+
+// One operand's way to LDS: kLoads instructions per wave and step
+template <typename T, int LAYOUT, int ROWS, int WAVES>
+struct Stream {
+  typedef Tile<T, LAYOUT, ROWS> Shape;
+  static constexpr int E = Shape::E;
+  static constexpr int kLoads = ROWS * 8 / (WAVES * 64);
+  const T* base;
+  long long ld;
+  uint32_t offset[kLoads], chunk_k[kLoads];
+  uint32_t extent;  // K_ADJACENT: bytes from the tile's first to its last element
+  uint32_t rows;    // ROW_ADJACENT: of the operand from the tile's first on
+
+  __device__ __forceinline__ Stream(const void* p, long long ld_, long long row0, long long I,
+                                    long long K, uint32_t wave, uint32_t lane) {
+    ld = ld_;
+    const uint32_t high = (uint32_t)min((long long)ROWS, I - row0);
+    rows = high;
+    if constexpr (LAYOUT == K_ADJACENT) {
+      base = (const T*)p + row0 * ld;
+      extent = (uint32_t)(((high - 1) * ld + K) * sizeof(T));
+    } else {
+      base = (const T*)p + row0;
+      extent = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < kLoads; ++n) {
+      const uint32_t q = (n * WAVES + wave) * 64 + lane;
+      const uint32_t line = q / Shape::kLine, slot = q % Shape::kLine;
+      if constexpr (LAYOUT == K_ADJACENT) {
+        const uint32_t c = slot ^ (line & 7);
+        chunk_k[n] = c * E;
+        offset[n] = line < high ? (uint32_t)(line * ld * sizeof(T)) + c * 16 : kOutside;
+      } else {
+        const uint32_t c = sizeof(T) == 2 ? slot ^ (4 * (line & 3)) : slot;
+        offset[n] = c * E < high ? (uint32_t)(line * ld * sizeof(T)) + c * 16 : kOutside;
+      }
+    }
+  }
+
+  // the step's k: k .. k + kDepth - 1, those from K on are zeros
+  __device__ __forceinline__ void load(uint32_t lds, long long k, long long K,
+                                       uint32_t wave) const {
+    if constexpr (LAYOUT == K_ADJACENT) {
+      const u32x4 buffer = buffer_of(base, extent);
+      const uint32_t at = (uint32_t)(k * sizeof(T));
+      const bool whole = k + Shape::kDepth <= K;
+      const uint32_t left = (uint32_t)(K - k);
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n) {
+        const uint32_t o = whole || chunk_k[n] < left ? offset[n] : kOutside;
+        chunks_to_lds(lds + (n * WAVES + wave) * 1024, o, buffer, at);
+      }
+    } else {
+      const uint32_t lines = (uint32_t)min((long long)Shape::kDepth, K - k);
+      const u32x4 buffer =
+          buffer_of(base + k * ld, (uint32_t)(((lines - 1) * ld + rows) * sizeof(T)));
+#pragma unroll
+      for (int n = 0; n < kLoads; ++n)
+        chunks_to_lds(lds + (n * WAVES + wave) * 1024, offset[n], buffer, 0);
+    }
+  }
+};
+
+// WI x WJ waves of XI x XJ blocks of 32 x 32
+template <typename T, int AL, int BL, int WI, int WJ, int XI, int XJ>
+__global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a) {
+  constexpr int kWaves = WI * WJ, kRows = WI * XI * 32, kCols = WJ * XJ * 32;
+  typedef Tile<T, AL, kRows> TA;
+  typedef Tile<T, BL, kCols> TB;
+  constexpr int kStage = TA::kBytes + TB::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  uint32_t i_tile, j_tile;
+  tile_of(blockIdx.x, a.ti, a.tj, &i_tile, &j_tile);
+  const long long i0 = (long long)i_tile * kRows, j0 = (long long)j_tile * kCols;
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t wi = wave / WJ * XI * 32, wj = wave % WJ * XJ * 32;
+  const long long k_begin = blockIdx.y * a.k_part;
+  const long long k_end = min(a.K, k_begin + a.k_part);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+  const Stream<T, AL, kRows, kWaves> sa(a.a, a.lda, i0, a.I, a.K, wave, lane);
+  const Stream<T, BL, kCols, kWaves> sb(a.b, a.ldb, j0, a.J, a.K, wave, lane);
+
+  f32x16 acc[XI][XJ];
+#pragma unroll
+  for (int x = 0; x < XI; ++x)
+#pragma unroll
+    for (int y = 0; y < XJ; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
+
+  sa.load(lds0, k_begin, k_end, wave);
+  sb.load(lds0 + TA::kBytes, k_begin, k_end, wave);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  uint32_t now = 0;
+  for (long long k = k_begin; k < k_end; k += TA::kDepth, now ^= kStage) {
+    if (k + TA::kDepth < k_end) {  // into the half that everyone has left at the last barrier
+      sa.load(lds0 + (now ^ kStage), k + TA::kDepth, k_end, wave);
+      sb.load(lds0 + (now ^ kStage) + TA::kBytes, k + TA::kDepth, k_end, wave);
+    }
+    const char* la = lds + now;
+    const char* lb = la + TA::kBytes;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      u32x4 fa[XI], fb[XJ];
+#pragma unroll
+      for (int x = 0; x < XI; ++x) fa[x] = TA::fragment(la, wi + 32 * x, s, lane);
+#pragma unroll
+      for (int y = 0; y < XJ; ++y) fb[y] = TB::fragment(lb, wj + 32 * y, s, lane);
+#pragma unroll
+      for (int x = 0; x < XI; ++x)
+#pragma unroll
+        for (int y = 0; y < XJ; ++y) acc[x][y] = Mfma<T>::run(fb[y], fa[x], acc[x][y]);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the next step's chunks are in LDS
+    __syncthreads();
+  }
+
+  // sums through LDS as above, kSlab rows at a time
+  constexpr uint32_t kSlab = 2 * kStage / (kCols * 4), kQuads = kCols / 4;
+  const uint32_t c = threadIdx.x % kQuads;
+  const long long j = j0 + c * 4;
+  const int n = (int)min(4ll, a.J - j);
+#pragma unroll
+  for (uint32_t slab = 0; slab < kRows; slab += kSlab) {
+    if (slab) __syncthreads();
+    if (wi >= slab && wi < slab + kSlab) {
+#pragma unroll
+      for (int x = 0; x < XI; ++x) {
+#pragma unroll
+        for (int y = 0; y < XJ; ++y) {
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const uint32_t i = wi - slab + 32 * x + lane % 32;
+            const uint32_t q = (wj + 32 * y + 8 * g) / 4 + lane / 32;
+            const f32x4 v = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2],
+                             acc[x][y][4 * g + 3]};
+            *reinterpret_cast<f32x4*>(lds + (i * kQuads + (q ^ (i & 31))) * 16) = v;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const long long left = a.I - i0 - slab;
+    const uint32_t high = left < 0 ? 0u : (uint32_t)min((long long)kSlab, left);
+    if (n > 0) {
+#pragma unroll 1
+      for (uint32_t i = threadIdx.x / kQuads; i < high; i += kWaves * 64 / kQuads) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (i * kQuads + (c ^ (i & 31))) * 16);
+        if (a.e.partial) {
+          float* p = a.e.partial + ((long long)blockIdx.y * a.I + i0 + slab + i) * a.J + j;
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < n) p[q] = v[q];
+        } else {
+          finish<T>(a.e, i0 + slab + i, j, n, v);
+        }
+      }
+    }
+  }
+}
+
 // The parts of a K that was split, in order, then the epilogue.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, uint32_t split,
@@ -527,15 +719,30 @@ constexpr int kUnits = 256;  // compute units to fill
 struct Product {
   uint32_t ti, tj, split;
   long long k_part;
+  int edge;     // rows and columns of a tile
+  bool direct;  // stream_kernel (both operands aligned) or tile_kernel
   long long bytes(long long I, long long J) const {
     return split > 1 ? (long long)split * I * J * 4 : 0;
   }
 };
 
+// An operand that stream_kernel can take: every 16-byte chunk aligned and not across an end,
+// a tile's offsets below 2^31.
+bool streamable(const void* p, long long ld, int layout, long long rows, long long K, int size) {
+  const int e = 16 / size;
+  if (((uintptr_t)p & 15) || ld % e || ld * size > (1 << 22)) return false;
+  return layout == K_ADJACENT ? K % e == 0 && K * size <= (1 << 22) && ld >= 0
+                              : rows % e == 0 && ld >= rows;
+}
+
 // K is split where the tiles alone leave compute units idle, into parts of at least four
 // steps (512 bytes of k).
-bool plan_product(long long I, long long J, long long K, int dtype, Product* p) {
-  const long long ti = (I + 127) / 128, tj = (J + 127) / 128;
+bool plan_product(long long I, long long J, long long K, int dtype, bool direct, Product* p) {
+  p->direct = direct;
+  p->edge = 128;
+  if (direct && dtype != TEMPO_DTYPE_F32 && (I + 255) / 256 * ((J + 255) / 256) >= kUnits)
+    p->edge = 256;
+  const long long ti = (I + p->edge - 1) / p->edge, tj = (J + p->edge - 1) / p->edge;
   if (ti > 0x3fffffff / tj) return false;
   p->ti = (uint32_t)ti;
   p->tj = (uint32_t)tj;
@@ -550,17 +757,39 @@ bool plan_product(long long I, long long J, long long K, int dtype, Product* p) 
   return p->split <= 65535;
 }
 
+// Scratch memory is planned from sizes alone: either kernel may run in the end.
+bool product_bytes(long long I, long long J, long long K, int dtype, long long* bytes) {
+  Product a, b;
+  if (!plan_product(I, J, K, dtype, false, &a) || !plan_product(I, J, K, dtype, true, &b))
+    return false;
+  const long long x = a.bytes(I, J), y = b.bytes(I, J);
+  *bytes = x > y ? x : y;
+  return true;
+}
+
 template <typename T, int AL, int BL>
-int run_product(const Product& p, const void* a, long long lda, const void* b, long long ldb,
-                long long I, long long J, long long K, const Epilogue& e, float* scratch,
+int run_product(const void* a, long long lda, const void* b, long long ldb, long long I,
+                long long J, long long K, const Epilogue& e, float* scratch,
                 hipStream_t stream) {
+  constexpr int dtype = sizeof(T) == 4 ? TEMPO_DTYPE_F32 : TEMPO_DTYPE_F16;
+  Product p;
+  plan_product(I, J, K, dtype,
+               streamable(a, lda, AL, I, K, sizeof(T)) && streamable(b, ldb, BL, J, K, sizeof(T)),
+               &p);
   TileArgs t = {};
   t.a = a; t.b = b; t.lda = lda; t.ldb = ldb; t.I = I; t.J = J; t.K = K;
   t.ti = p.ti; t.tj = p.tj; t.split = p.split; t.k_part = p.k_part;
   t.e = e;
   t.e.partial = p.split > 1 ? scratch : nullptr;
-  hipLaunchKernelGGL((tile_kernel<T, AL, BL>), dim3(p.ti * p.tj, p.split), dim3(kThreads), 0,
-                     stream, t);
+  const dim3 grid(p.ti * p.tj, p.split);
+  if (!p.direct) {
+    hipLaunchKernelGGL((tile_kernel<T, AL, BL>), grid, dim3(kThreads), 0, stream, t);
+  } else if (p.edge == 128) {
+    hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2>), grid, dim3(256), 0, stream, t);
+  } else {
+    if constexpr (sizeof(T) == 2)
+      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 4, 4, 2>), grid, dim3(512), 0, stream, t);
+  }
   if (p.split > 1) {
     const long long quads = I * ((J + 3) / 4);
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((quads + kThreads - 1) / kThreads)),
@@ -570,7 +799,6 @@ int run_product(const Product& p, const void* a, long long lda, const void* b, l
 }
 
 struct BackwardPlan {
-  Product dx, dw;
   long long dz_bytes, sum_bytes, scratch_bytes;
   long long total() const { return dz_bytes + sum_bytes + scratch_bytes; }
 };
@@ -578,11 +806,10 @@ struct BackwardPlan {
 long long up16(long long n) { return (n + 15) / 16 * 16; }
 
 bool plan_backward(long long M, int N, int K, int dtype, int act, BackwardPlan* p) {
-  if (!plan_product(M, K, N, dtype, &p->dx) || !plan_product(N, K, M, dtype, &p->dw))
-    return false;
+  long long x, w;
+  if (!product_bytes(M, K, N, dtype, &x) || !product_bytes(N, K, M, dtype, &w)) return false;
   p->dz_bytes = act == NONE ? 0 : up16(M * N * (dtype == TEMPO_DTYPE_F32 ? 4 : 2));
   p->sum_bytes = up16((M + kRowsPerBlock - 1) / kRowsPerBlock * N * 4);
-  const long long x = p->dx.bytes(M, K), w = p->dw.bytes(N, K);
   p->scratch_bytes = up16(x > w ? x : w);
   return true;
 }
@@ -598,13 +825,6 @@ int check_sizes(long long M, int N, int K, int dtype, int act) {
 
 bool misaligned(const void* p, int dtype) {
   return ((uintptr_t)p & (dtype == TEMPO_DTYPE_F32 ? 3 : 1)) != 0;
-}
-
-template <typename T>
-int forward_for(const Product& p, const void* x, long long ldx, const void* w, long long ldw,
-                const Epilogue& e, long long M, int N, int K, float* scratch,
-                hipStream_t stream) {
-  return run_product<T, K_ADJACENT, K_ADJACENT>(p, x, ldx, w, ldw, M, N, K, e, scratch, stream);
 }
 
 template <typename T>
@@ -629,13 +849,11 @@ int backward_for(const BackwardPlan& p, const void* g, long long ldg, const void
   int rc = (int)hipGetLastError();
   if (rc == 0 && dx) {
     e.out = dx; e.ldo = lddx;
-    rc = run_product<T, K_ADJACENT, ROW_ADJACENT>(p.dx, z, ldz, w, ldw, M, K, N, e, scratch,
-                                                  stream);
+    rc = run_product<T, K_ADJACENT, ROW_ADJACENT>(z, ldz, w, ldw, M, K, N, e, scratch, stream);
   }
   if (rc == 0 && dw) {
     e.out = dw; e.ldo = K;
-    rc = run_product<T, ROW_ADJACENT, ROW_ADJACENT>(p.dw, z, ldz, x, ldx, N, K, M, e, scratch,
-                                                    stream);
+    rc = run_product<T, ROW_ADJACENT, ROW_ADJACENT>(z, ldz, x, ldx, N, K, M, e, scratch, stream);
   }
   return rc;
 }
@@ -652,8 +870,8 @@ long long tempo_linear_workspace(long long M, int N, int K, int dtype, int activ
     BackwardPlan p;
     return plan_backward(M, N, K, dtype, activation, &p) ? p.total() : TEMPO_E_SIZE;
   }
-  Product p;
-  return plan_product(M, N, K, dtype, &p) ? p.bytes(M, N) : TEMPO_E_SIZE;
+  long long bytes;
+  return product_bytes(M, N, K, dtype, &bytes) ? bytes : TEMPO_E_SIZE;
 }
 
 int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw,
@@ -663,13 +881,12 @@ int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw
   if (!x || !weight || !y) return TEMPO_E_NULL;
   const int rc = check_sizes(M, N, K, dtype, activation);
   if (rc != TEMPO_OK) return rc;
-  Product p;
-  if (!plan_product(M, N, K, dtype, &p)) return TEMPO_E_SIZE;
+  long long need;
+  if (!product_bytes(M, N, K, dtype, &need)) return TEMPO_E_SIZE;
   if (ldx < 0 || ldw < 0 || ldr < 0 || (M > 1 && ldy < N)) return TEMPO_E_ARG;
   if (misaligned(x, dtype) || misaligned(weight, dtype) || misaligned(y, dtype) ||
       misaligned(bias, dtype) || misaligned(residual, dtype) || misaligned(pre, dtype))
     return TEMPO_E_ARG;
-  const long long need = p.bytes(M, N);
   if (need > 0 && !workspace) return TEMPO_E_NULL;
   if (need > workspace_bytes) return TEMPO_E_SIZE;
   if ((uintptr_t)workspace & 15) return TEMPO_E_ARG;
@@ -679,10 +896,11 @@ int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw
   float* scratch = (float*)workspace;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == TEMPO_DTYPE_F32)
-    return forward_for<float>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
+    return run_product<float, K_ADJACENT, K_ADJACENT>(x, ldx, weight, ldw, M, N, K, e, scratch, s);
   if (dtype == TEMPO_DTYPE_F16)
-    return forward_for<_Float16>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
-  return forward_for<__bf16>(p, x, ldx, weight, ldw, e, M, N, K, scratch, s);
+    return run_product<_Float16, K_ADJACENT, K_ADJACENT>(x, ldx, weight, ldw, M, N, K, e, scratch,
+                                                         s);
+  return run_product<__bf16, K_ADJACENT, K_ADJACENT>(x, ldx, weight, ldw, M, N, K, e, scratch, s);
 }
 
 int tempo_linear_backward(const void* grad_y, long long ldg, const void* pre, const void* x,

@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kSpan = TEMPO_RECURRENCE_SPAN;
+constexpr int kBatch = 8;          // steps loaded at a time; divides kSpan
 constexpr int kScanLanes = 16;     // pass 2: lanes x segments of a workgroup
 constexpr int kScanSegments = 64;
 
@@ -58,10 +59,15 @@ struct RecurrenceArgs {
   uint32_t lanes, chunk, nchunk;  // lanes = B * DV
 };
 
-// One thread's place: V neighbouring channels of one batch row, one chunk of time.
+// One thread's place: V neighbouring channels of one batch row, one chunk of time.  Where V
+// does not divide D, the last lane of a row moves back so that its V channels are inside the
+// row, too: it shares `skip` of them with its neighbour and stores the others alone (a lane
+// that loaded its few channels one by one would hold up its wave: 294 against 92 us for the
+// backward pass of 13 x 4097 x 771 in fp16).
+// Rows of fewer than V channels (n < V) go channel by channel.
 template <int V>
 struct Place {
-  uint32_t lane, b, d, n, c;  // n <= V channels are inside the row
+  uint32_t lane, b, d, n, c, skip;
   bool on;
   __device__ Place(const RecurrenceArgs& a) {
     const uint32_t id = blockIdx.x * kBlock + threadIdx.x;
@@ -69,26 +75,32 @@ struct Place {
     c = id / a.lanes;
     lane = id - c * a.lanes;
     b = lane / a.DV;
-    d = (lane - b * a.DV) * V;
-    n = min((uint32_t)V, a.D - d);
+    const uint32_t first = (lane - b * a.DV) * V;
+    n = min((uint32_t)V, a.D);
+    d = min(first, a.D - n);
+    skip = first - d;
   }
 };
 
-template <int V, typename T>
-__device__ __forceinline__ void load(const T* p, uint32_t n, float (&x)[V]) {
-  if (n == V) {
-    const typename Pack<T, V>::type r = *reinterpret_cast<const typename Pack<T, V>::type*>(p);
+// V channels as they lie in memory; FULL: all of them are inside the row
+template <bool FULL, int V, typename T>
+__device__ __forceinline__ typename Pack<T, V>::type fetch(const T* p, uint32_t n) {
+  if constexpr (FULL) return *reinterpret_cast<const typename Pack<T, V>::type*>(p);
+  typename Pack<T, V>::type r;
 #pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = (float)r[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = (uint32_t)j < n ? (float)p[j] : 0.f;
-  }
+  for (int j = 0; j < V; ++j) r[j] = (uint32_t)j < n ? p[j] : (T)0.f;
+  return r;
 }
 
-template <int V, typename T>
-__device__ __forceinline__ void store(T* p, uint32_t n, const float (&x)[V]) {
-  if (n == V) {
+template <int V>
+__device__ __forceinline__ void load(const float* p, uint32_t n, float (&x)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) x[j] = (uint32_t)j < n ? p[j] : 0.f;
+}
+
+template <bool FULL, int V, typename T>
+__device__ __forceinline__ void put(T* p, const Place<V>& at, const float (&x)[V]) {
+  if (FULL && at.skip == 0) {
     typename Pack<T, V>::type r;
 #pragma unroll
     for (int j = 0; j < V; ++j) r[j] = (T)x[j];
@@ -96,7 +108,7 @@ __device__ __forceinline__ void store(T* p, uint32_t n, const float (&x)[V]) {
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if ((uint32_t)j < n) p[j] = (T)x[j];
+      if ((uint32_t)j >= at.skip && (uint32_t)j < at.n) p[j] = (T)x[j];
   }
 }
 
@@ -118,6 +130,13 @@ __device__ __forceinline__ float small_weight(float g) {
 __device__ __forceinline__ float step(float w, bool shut, float h, float v) {
   const float base = shut ? h : v, other = shut ? v : h;
   return fmaf(w, other - base, base);
+}
+
+// one more step of a chunk's A = k and S = 1 - A = s, each to its own full precision
+__device__ __forceinline__ void summarize(float w, bool shut, float* s, float* k) {
+  const float rest = 1.f - w;
+  *s = fmaf(shut ? w : rest, *k, *s);
+  *k *= shut ? rest : w;
 }
 
 // h_out of a chunk (or of several) from its incoming state
@@ -157,29 +176,37 @@ __device__ __forceinline__ void load_state(const float* p, const RecurrenceArgs&
 
 // ------------------------------------------------------------------------------- forward
 
-template <typename T, int V>
-__global__ __launch_bounds__(kBlock) void forward_summary_kernel(const RecurrenceArgs a) {
-  const Place<V> at(a);
-  if (!at.on) return;
+// kBatch steps are loaded at a time; the last batch of a chunk loads its last step again in
+// place of those that are missing.
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void forward_summary(const RecurrenceArgs& a, const Place<V>& at) {
   const uint32_t begin = at.c * a.chunk;
   const uint32_t end = min(begin + a.chunk, length_of(a, at.b));
-  const T* pg = (const T*)a.gate + at.b * a.gate_sb + at.d;
-  const T* pv = (const T*)a.value + at.b * a.value_sb + at.d;
+  const uint32_t steps = end > begin ? end - begin : 0;
+  const T* pg = (const T*)a.gate + (at.b * a.gate_sb + begin * a.gate_st + at.d);
+  const T* pv = (const T*)a.value + (at.b * a.value_sb + begin * a.value_st + at.d);
   float s[V], k[V], u[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = u[j] = 0.f, k[j] = 1.f;
-#pragma unroll 8
-  for (uint32_t t = begin; t < end; ++t) {
-    float g[V], v[V];
-    load<V>(pg + t * a.gate_st, at.n, g);
-    load<V>(pv + t * a.value_st, at.n, v);
+  for (uint32_t i = 0; i < steps; i += kBatch) {
+    typename Pack<T, V>::type g[kBatch], v[kBatch];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float w = small_weight<T>(g[j]);
-      const bool shut = g[j] < 0.f;
-      u[j] = step(w, shut, u[j], v[j]);
-      s[j] = step(w, shut, s[j], 1.f);
-      k[j] *= shut ? 1.f - w : w;
+    for (int q = 0; q < kBatch; ++q) {
+      const uint32_t t = min(i + q, steps - 1);
+      g[q] = fetch<FULL, V>(pg + t * a.gate_st, at.n);
+      v[q] = fetch<FULL, V>(pv + t * a.value_st, at.n);
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (i + q < steps) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float x = (float)g[q][j], w = small_weight<T>(x);
+          const bool shut = x < 0.f;
+          u[j] = step(w, shut, u[j], (float)v[q][j]);
+          summarize(w, shut, &s[j], &k[j]);
+        }
+      }
     }
   }
   const size_t o = ((size_t)at.c * a.lanes + at.lane) * V;
@@ -188,6 +215,14 @@ __global__ __launch_bounds__(kBlock) void forward_summary_kernel(const Recurrenc
     a.weight[o + j] = s[j] < 0.5f ? s[j] : -k[j];
     a.carry[o + j] = u[j];
   }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void forward_summary_kernel(const RecurrenceArgs a) {
+  const Place<V> at(a);
+  if (!at.on) return;
+  if (at.n == V) forward_summary<true, T, V>(a, at);
+  else forward_summary<false, T, V>(a, at);
 }
 
 // Pass 2 of both directions: chunk summaries -> every chunk's incoming value (over `carry`)
@@ -199,8 +234,10 @@ __global__ __launch_bounds__(kScanLanes* kScanSegments) void scan_kernel(const R
   const uint32_t l = threadIdx.x % kScanLanes, seg = threadIdx.x / kScanLanes;
   const uint32_t width = a.lanes * V;
   const uint32_t q = blockIdx.x * kScanLanes + l;
-  const uint32_t lane = q / V, b = lane / a.DV, d = (lane - b * a.DV) * V + q % V;
-  const bool on = q < width && d < a.D;
+  const uint32_t lane = q / V, b = lane / a.DV, d0 = (lane - b * a.DV) * V;
+  const uint32_t moved = d0 - min(d0, a.D - min((uint32_t)V, a.D));  // see Place
+  const uint32_t d = d0 - moved + q % V;
+  const bool on = q < width && q % V >= moved && d < a.D;
   const uint32_t run = (a.nchunk + kScanSegments - 1) / kScanSegments;
   const uint32_t first = min(seg * run, a.nchunk), stop = min(first + run, a.nchunk);
   float weight = 0.f, u = 0.f;
@@ -229,67 +266,93 @@ __global__ __launch_bounds__(kScanLanes* kScanSegments) void scan_kernel(const R
   if (seg == kScanSegments - 1 && a.last) a.last[(size_t)b * a.D + d] = h;
 }
 
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void forward_chunk(const RecurrenceArgs& a, const Place<V>& at) {
+  const uint32_t begin = at.c * a.chunk, stop = min(begin + a.chunk, a.T);
+  const uint32_t end = max(begin, min(stop, length_of(a, at.b)));
+  const uint32_t steps = end - begin, all = stop - begin;
+  const T* pg = (const T*)a.gate + (at.b * a.gate_sb + begin * a.gate_st + at.d);
+  const T* pv = (const T*)a.value + (at.b * a.value_sb + begin * a.value_st + at.d);
+  T* ph = (T*)a.out + (at.b * a.out_sb + begin * a.out_st + at.d);
+  const size_t row = (size_t)at.b * a.D + at.d, width = (size_t)a.B * a.D;
+  float* ckpt = a.ckpt ? a.ckpt + (begin / kSpan) * width + row : nullptr;
+  float h[V];
+  if (a.nchunk > 1)
+    load<V>(a.carry + ((size_t)at.c * a.lanes + at.lane) * V, V, h);
+  else
+    load_state<V>(a.state, a, at.b, at.d, at.n, h);
+  for (uint32_t i = 0; i < steps; i += kBatch) {
+    typename Pack<T, V>::type g[kBatch], v[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const uint32_t t = min(i + q, steps - 1);
+      g[q] = fetch<FULL, V>(pg + t * a.gate_st, at.n);
+      v[q] = fetch<FULL, V>(pv + t * a.value_st, at.n);
+    }
+    if (ckpt && i % kSpan == 0) {
+      put<FULL, V>(ckpt, at, h);
+      ckpt += width;
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (i + q < steps) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float x = (float)g[q][j];
+          h[j] = step(small_weight<T>(x), x < 0.f, h[j], (float)v[q][j]);
+        }
+        put<FULL, V>(ph + (i + q) * a.out_st, at, h);
+      }
+    }
+  }
+  if (a.nchunk == 1 && a.last) put<FULL, V>(a.last + row, at, h);
+#pragma unroll
+  for (int j = 0; j < V; ++j) h[j] = 0.f;
+  for (uint32_t i = steps; i < all; ++i) put<FULL, V>(ph + i * a.out_st, at, h);
+}
+
 template <typename T, int V>
 __global__ __launch_bounds__(kBlock) void forward_kernel(const RecurrenceArgs a) {
   const Place<V> at(a);
   if (!at.on) return;
-  const uint32_t begin = at.c * a.chunk, stop = min(begin + a.chunk, a.T);
-  const uint32_t end = max(begin, min(stop, length_of(a, at.b)));
-  const T* pg = (const T*)a.gate + at.b * a.gate_sb + at.d;
-  const T* pv = (const T*)a.value + at.b * a.value_sb + at.d;
-  T* ph = (T*)a.out + at.b * a.out_sb + at.d;
-  const size_t row = (size_t)at.b * a.D + at.d, width = (size_t)a.B * a.D;
-  float h[V];
-  if (a.nchunk > 1) {
-    const float* p = a.carry + ((size_t)at.c * a.lanes + at.lane) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) h[j] = p[j];
-  } else {
-    load_state<V>(a.state, a, at.b, at.d, at.n, h);
-  }
-#pragma unroll 8
-  for (uint32_t t = begin; t < end; ++t) {
-    if (a.ckpt && t % kSpan == 0) store<V>(a.ckpt + (t / kSpan) * width + row, at.n, h);
-    float g[V], v[V];
-    load<V>(pg + t * a.gate_st, at.n, g);
-    load<V>(pv + t * a.value_st, at.n, v);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      h[j] = step(small_weight<T>(g[j]), g[j] < 0.f, h[j], v[j]);
-    store<V>(ph + t * a.out_st, at.n, h);
-  }
-  if (a.nchunk == 1 && a.last) store<V>(a.last + row, at.n, h);
-#pragma unroll
-  for (int j = 0; j < V; ++j) h[j] = 0.f;
-  for (uint32_t t = end; t < stop; ++t) store<V>(ph + t * a.out_st, at.n, h);
+  if (at.n == V) forward_chunk<true, T, V>(a, at);
+  else forward_chunk<false, T, V>(a, at);
 }
 
 // ------------------------------------------------------------------------------ backward
 
-template <typename T, int V>
-__global__ __launch_bounds__(kBlock) void backward_summary_kernel(const RecurrenceArgs a) {
-  const Place<V> at(a);
-  if (!at.on) return;
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void backward_summary(const RecurrenceArgs& a, const Place<V>& at) {
   const uint32_t begin = at.c * a.chunk;
   const uint32_t end = max(begin, min(begin + a.chunk, length_of(a, at.b)));
-  const T* pg = (const T*)a.gate + at.b * a.gate_sb + at.d;
-  const T* pe = (const T*)a.grad_h + at.b * a.grad_sb + at.d;
+  const uint32_t steps = end - begin;
+  // from the last step of the chunk back
+  const long long from = (long long)end - 1;
+  const T* pg = (const T*)a.gate + (at.b * a.gate_sb + from * a.gate_st + at.d);
+  const T* pe = (const T*)a.grad_h + (at.b * a.grad_sb + from * a.grad_st + at.d);
   float s[V], k[V], p[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = p[j] = 0.f, k[j] = 1.f;
-#pragma unroll 8
-  for (uint32_t t = end; t-- > begin;) {
-    float g[V], e[V];
-    load<V>(pg + t * a.gate_st, at.n, g);
-    load<V>(pe + t * a.grad_st, at.n, e);
+  for (uint32_t i = 0; i < steps; i += kBatch) {
+    typename Pack<T, V>::type g[kBatch], e[kBatch];
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float w = small_weight<T>(g[j]);
-      const bool shut = g[j] < 0.f;
-      const float x = e[j] + p[j], wx = w * x;
-      p[j] = shut ? x - wx : wx;
-      s[j] = step(w, shut, s[j], 1.f);
-      k[j] *= shut ? 1.f - w : w;
+    for (int q = 0; q < kBatch; ++q) {
+      const uint32_t t = min(i + q, steps - 1);
+      g[q] = fetch<FULL, V>(pg - t * a.gate_st, at.n);
+      e[q] = fetch<FULL, V>(pe - t * a.grad_st, at.n);
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      if (i + q < steps) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float y = (float)g[q][j], w = small_weight<T>(y);
+          const bool shut = y < 0.f;
+          const float x = (float)e[q][j] + p[j], wx = w * x;
+          p[j] = shut ? x - wx : wx;
+          summarize(w, shut, &s[j], &k[j]);
+        }
+      }
     }
   }
   const size_t o = ((size_t)at.c * a.lanes + at.lane) * V;
@@ -300,90 +363,114 @@ __global__ __launch_bounds__(kBlock) void backward_summary_kernel(const Recurren
   }
 }
 
-// A span of C steps at a time, last span first: recompute its states from the checkpoint
-// and keep per step w (negative where the gate is open) and z f (v - h); then walk it back.
+template <typename T, int V>
+__global__ __launch_bounds__(kBlock) void backward_summary_kernel(const RecurrenceArgs a) {
+  const Place<V> at(a);
+  if (!at.on) return;
+  if (at.n == V) backward_summary<true, T, V>(a, at);
+  else backward_summary<false, T, V>(a, at);
+}
+
+// A span of C steps: recompute its states from the checkpoint, keep per step w (negative
+// where the gate is open) and z f (v - h); then walk it back.
+template <bool FULL, bool WHOLE, typename T, int V, int C>
+__device__ __forceinline__ void backward_span(const RecurrenceArgs& a, const Place<V>& at,
+                                              uint32_t t0, uint32_t steps, const T* pg,
+                                              const T* pv, const T* pe, T* pdg, T* pdv,
+                                              float (&p)[V]) {
+  typename Pack<T, V>::type g[C], v[C], e[C];
+  const uint32_t last = WHOLE ? C - 1 : steps - 1;
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const uint32_t t = WHOLE ? k : min((uint32_t)k, last);
+    g[k] = fetch<FULL, V>(pg + t * a.gate_st, at.n);
+    v[k] = fetch<FULL, V>(pv + t * a.value_st, at.n);
+  }
+  float w[C][V], r[C][V], h[V];
+  if (a.ckpt_in) {
+    const size_t row = (size_t)at.b * a.D + at.d, width = (size_t)a.B * a.D;
+    load<V>(a.ckpt_in + (t0 / kSpan) * width + row, at.n, h);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) h[j] = 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    const uint32_t t = WHOLE ? k : min((uint32_t)k, last);
+    e[k] = fetch<FULL, V>(pe + t * a.grad_st, at.n);
+  }
+#pragma unroll
+  for (int k = 0; k < C; ++k) {
+    if (WHOLE || (uint32_t)k < steps) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float y = (float)g[k][j], x = small_weight<T>(y), z = (float)v[k][j];
+        const bool shut = y < 0.f;
+        w[k][j] = shut ? x : -x;
+        r[k][j] = (x - x * x) * (z - h[j]);
+        h[j] = step(x, shut, h[j], z);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = C - 1; k >= 0; --k) {
+    if (WHOLE || (uint32_t)k < steps) {
+      float dg[V], dv[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float x = (float)e[k][j] + p[j], wx = fabsf(w[k][j]) * x;
+        const bool shut = !(__float_as_uint(w[k][j]) >> 31);
+        dg[j] = r[k][j] * x;
+        dv[j] = shut ? wx : x - wx;
+        p[j] = shut ? x - wx : wx;
+      }
+      put<FULL, V>(pdg + k * a.out_st, at, dg);
+      put<FULL, V>(pdv + k * a.out2_st, at, dv);
+    }
+  }
+}
+
+template <bool FULL, typename T, int V, int C>
+__device__ __forceinline__ void backward_chunk(const RecurrenceArgs& a, const Place<V>& at) {
+  const uint32_t begin = at.c * a.chunk, stop = min(begin + a.chunk, a.T);
+  const uint32_t end = max(begin, min(stop, length_of(a, at.b)));
+  const T* pg = (const T*)a.gate + (at.b * a.gate_sb + begin * a.gate_st + at.d);
+  const T* pv = (const T*)a.value + (at.b * a.value_sb + begin * a.value_st + at.d);
+  const T* pe = (const T*)a.grad_h + (at.b * a.grad_sb + begin * a.grad_st + at.d);
+  T* pdg = (T*)a.out + (at.b * a.out_sb + begin * a.out_st + at.d);
+  T* pdv = (T*)a.out2 + (at.b * a.out2_sb + begin * a.out2_st + at.d);
+  float p[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) p[j] = 0.f;
+  for (uint32_t i = end - begin; i < stop - begin; ++i) {
+    put<FULL, V>(pdg + i * a.out_st, at, p);
+    put<FULL, V>(pdv + i * a.out2_st, at, p);
+  }
+  if (a.nchunk > 1)
+    load<V>(a.carry + ((size_t)at.c * a.lanes + at.lane) * V, V, p);
+  else
+    load_state<V>(a.state, a, at.b, at.d, at.n, p);
+  const uint32_t steps = end - begin, rest = steps % C;
+  uint32_t i = steps - rest;
+  if (rest)
+    backward_span<FULL, false, T, V, C>(a, at, begin + i, rest, pg + i * a.gate_st,
+                                        pv + i * a.value_st, pe + i * a.grad_st,
+                                        pdg + i * a.out_st, pdv + i * a.out2_st, p);
+  while (i > 0) {
+    i -= C;
+    backward_span<FULL, true, T, V, C>(a, at, begin + i, C, pg + i * a.gate_st,
+                                       pv + i * a.value_st, pe + i * a.grad_st,
+                                       pdg + i * a.out_st, pdv + i * a.out2_st, p);
+  }
+  if (a.nchunk == 1 && a.last) put<FULL, V>(a.last + (size_t)at.b * a.D + at.d, at, p);
+}
+
 template <typename T, int V, int C>
 __global__ __launch_bounds__(kBlock) void backward_kernel(const RecurrenceArgs a) {
   const Place<V> at(a);
   if (!at.on) return;
-  const uint32_t begin = at.c * a.chunk, stop = min(begin + a.chunk, a.T);
-  const uint32_t end = max(begin, min(stop, length_of(a, at.b)));
-  const T* pg = (const T*)a.gate + at.b * a.gate_sb + at.d;
-  const T* pv = (const T*)a.value + at.b * a.value_sb + at.d;
-  const T* pe = a.grad_h ? (const T*)a.grad_h + at.b * a.grad_sb + at.d : nullptr;
-  T* pdg = (T*)a.out + at.b * a.out_sb + at.d;
-  T* pdv = (T*)a.out2 + at.b * a.out2_sb + at.d;
-  const size_t row = (size_t)at.b * a.D + at.d, width = (size_t)a.B * a.D;
-  float p[V];
-  if (a.nchunk > 1) {
-    const float* c = a.carry + ((size_t)at.c * a.lanes + at.lane) * V;
-#pragma unroll
-    for (int j = 0; j < V; ++j) p[j] = c[j];
-  } else {
-    load_state<V>(a.state, a, at.b, at.d, at.n, p);
-  }
-  {
-    float zero[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) zero[j] = 0.f;
-    for (uint32_t t = end; t < stop; ++t) {
-      store<V>(pdg + t * a.out_st, at.n, zero);
-      store<V>(pdv + t * a.out2_st, at.n, zero);
-    }
-  }
-  const uint32_t spans = (end - begin + C - 1) / C;
-  for (uint32_t i = spans; i-- > 0;) {
-    const uint32_t t0 = begin + i * C;
-    const uint32_t left = end - t0;  // > 0; steps beyond it are not taken
-    float w[C][V], r[C][V], h[V];
-    if (a.ckpt_in) {
-      load<V>(a.ckpt_in + (t0 / kSpan) * width + row, at.n, h);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) h[j] = 0.f;
-    }
-#pragma unroll
-    for (int k = 0; k < C; ++k) {
-      if ((uint32_t)k < left) {
-        const uint32_t t = t0 + k;
-        float g[V], v[V];
-        load<V>(pg + t * a.gate_st, at.n, g);
-        load<V>(pv + t * a.value_st, at.n, v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float x = small_weight<T>(g[j]);
-          const bool shut = g[j] < 0.f;
-          w[k][j] = shut ? x : -x;
-          r[k][j] = (x - x * x) * (v[j] - h[j]);
-          h[j] = step(x, shut, h[j], v[j]);
-        }
-      }
-    }
-#pragma unroll
-    for (int k = C - 1; k >= 0; --k) {
-      if ((uint32_t)k < left) {
-        const uint32_t t = t0 + k;
-        float e[V], dg[V], dv[V];
-        if (pe) {
-          load<V>(pe + t * a.grad_st, at.n, e);
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) e[j] = 0.f;
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float x = e[j] + p[j], wx = fabsf(w[k][j]) * x;
-          const bool shut = !(__float_as_uint(w[k][j]) >> 31);
-          dg[j] = r[k][j] * x;
-          dv[j] = shut ? wx : x - wx;
-          p[j] = shut ? x - wx : wx;
-        }
-        store<V>(pdg + t * a.out_st, at.n, dg);
-        store<V>(pdv + t * a.out2_st, at.n, dv);
-      }
-    }
-  }
-  if (a.nchunk == 1 && a.last) store<V>(a.last + row, at.n, p);
+  if (at.n == V) backward_chunk<true, T, V, C>(a, at);
+  else backward_chunk<false, T, V, C>(a, at);
 }
 
 // --------------------------------------------------------------------------------- host
@@ -393,13 +480,15 @@ struct Plan {
   uint32_t lanes, DV, chunk, nchunk;
 };
 
-// Threads hold 4 channels (backward in fp32: 2, its registers hold a span of fp32 values).
-// Time is cut only where the (b, d) lanes alone are fewer than kFill threads.
-constexpr uint32_t kFill = 1u << 17;
+// Threads hold 4 channels; the backward beyond 4 steps 2, for its registers hold a span of
+// fp32 values (8 x 2048 x 1024 in bf16: 34 us against 42 with 4, 256 registers).  Time is cut
+// only where the (b, d) lanes alone are fewer than kFill threads, 16 waves for each of the
+// 256 compute units' 4 SIMDs (1 x 65536 x 1024: 68 us for the last pass, 80 with half of that).
+constexpr uint32_t kFill = 1u << 18;
 constexpr uint32_t kMinChunk = 2 * kSpan;
 
-bool make_plan(long long B, int T, int D, int dtype, bool backward, Plan* p) {
-  p->vec = backward && dtype == TEMPO_DTYPE_F32 && T > 4 ? 2 : 4;
+bool make_plan(long long B, int T, int D, bool backward, Plan* p) {
+  p->vec = backward && T > 4 ? 2 : 4;
   p->DV = (uint32_t)((D + p->vec - 1) / p->vec);
   const long long lanes = B * p->DV;
   if (lanes > 0x7fffffffLL) return false;
@@ -462,9 +551,8 @@ int launch_backward(const RecurrenceArgs& a, hipStream_t stream) {
 
 template <typename T>
 int launch_backward_for(const RecurrenceArgs& a, int vec, hipStream_t stream) {
-  if (a.T <= 4) return launch_backward<T, 4, 4>(a, stream);
-  if (vec == 2) return launch_backward<T, 2, kSpan>(a, stream);
-  return launch_backward<T, 4, kSpan>(a, stream);
+  if (vec == 4) return launch_backward<T, 4, 4>(a, stream);
+  return launch_backward<T, 2, kSpan>(a, stream);
 }
 
 }  // namespace
@@ -475,7 +563,7 @@ long long tempo_recurrence_workspace(long long B, int T, int D, int dtype, int b
   const int rc = check_sizes(B, T, D, dtype);
   if (rc != TEMPO_OK) return rc;
   Plan p;
-  if (!make_plan(B, T, D, dtype, backward != 0, &p)) return TEMPO_E_SIZE;
+  if (!make_plan(B, T, D, backward != 0, &p)) return TEMPO_E_SIZE;
   return plan_bytes(p);
 }
 
@@ -488,7 +576,7 @@ int tempo_recurrence(const void* gate, long long gate_sb, long long gate_st, con
   const int rc = check_sizes(B, T, D, dtype);
   if (rc != TEMPO_OK) return rc;
   Plan p;
-  if (!make_plan(B, T, D, dtype, false, &p)) return TEMPO_E_SIZE;
+  if (!make_plan(B, T, D, false, &p)) return TEMPO_E_SIZE;
   if (misaligned(gate, dtype) || misaligned(value, dtype) || misaligned(h, dtype))
     return TEMPO_E_ARG;
   const long long need = plan_bytes(p);
@@ -523,7 +611,7 @@ int tempo_recurrence_backward(const void* gate, long long gate_sb, long long gat
   if (rc != TEMPO_OK) return rc;
   if (!ckpt && T > kSpan) return TEMPO_E_NULL;
   Plan p;
-  if (!make_plan(B, T, D, dtype, true, &p)) return TEMPO_E_SIZE;
+  if (!make_plan(B, T, D, true, &p)) return TEMPO_E_SIZE;
   if (misaligned(gate, dtype) || misaligned(value, dtype) || misaligned(grad_h, dtype) ||
       misaligned(grad_gate, dtype) || misaligned(grad_value, dtype))
     return TEMPO_E_ARG;

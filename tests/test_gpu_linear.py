@@ -71,6 +71,15 @@ def test_gradients(shape, dtype, gpu_device):
         _check_grads(t, act, f'{act} ')
 
 
+@pytest.mark.parametrize('dtype', DTYPES[1:], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', [(4200, 72, 4104), (4104, 4104, 72), (72, 4104, 4104)], ids=str)
+def test_more_tiles_than_compute_units(shape, dtype, gpu_device):
+    """Each of the three products once large enough for the widest tiles, none of its sizes a
+    multiple of them."""
+    M, K, N = shape
+    _check_grads(_make(M, K, N, dtype, gpu_device, seed=4, residual=True, grad=True), 'silu')
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize('act', ACTS)
 def test_activations_over_their_range(act, dtype, gpu_device):
