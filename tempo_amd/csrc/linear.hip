@@ -202,7 +202,8 @@ __device__ __forceinline__ u32x4 load16(const T* p, long long left) {
 // One operand's tile in LDS: ROWS rows x 128 bytes of k.  16-byte chunks are permuted within
 // their row so that the reads below hit every bank equally:
 //   K_ADJACENT    [row][k]: chunk c of row r at c ^ (r % 8)
-//   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4);  fp32: as it is
+//   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4) (32 rows: as it is, four
+//                 lines are all banks already);  fp32: as it is
 template <typename T, int LAYOUT, int ROWS>
 struct Tile {
   static constexpr int E = 16 / sizeof(T);
@@ -211,13 +212,16 @@ struct Tile {
   static constexpr int kBytes = ROWS * 128;
   static constexpr int kPerThread = ROWS * 8 / kThreads;
 
-  static __device__ __forceinline__ uint32_t place(uint32_t line, uint32_t c) {
+  static __device__ __forceinline__ uint32_t swap(uint32_t line, uint32_t c) {
     if constexpr (LAYOUT == K_ADJACENT)
-      return (line * 8 + (c ^ (line & 7))) * 16;
-    else if constexpr (sizeof(T) == 2)
-      return (line * kLine + (c ^ (4 * (line & 3)))) * 16;
+      return c ^ (line & 7);
+    else if constexpr (sizeof(T) == 2 && ROWS >= 128)
+      return c ^ (4 * (line & 3));
     else
-      return (line * kLine + c) * 16;
+      return c;
+  }
+  static __device__ __forceinline__ uint32_t place(uint32_t line, uint32_t c) {
+    return (line * kLine + swap(line, c)) * 16;
   }
 
   static __device__ __forceinline__ void fetch(const T* p, long long ld, long long row0,
@@ -453,7 +457,7 @@ __device__ __forceinline__ void chunks_to_lds(uint32_t lds, uint32_t offset, u32
   asm volatile(
       "s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds),
       "v"(offset), "s"(buffer), "s"(scalar_offset)
-      : "memory", "m0");
+      : "memory");
 }
 
 // One operand's way to LDS: kLoads instructions per wave and step
@@ -485,11 +489,11 @@ struct Stream {
       const uint32_t q = (n * WAVES + wave) * 64 + lane;
       const uint32_t line = q / Shape::kLine, slot = q % Shape::kLine;
       if constexpr (LAYOUT == K_ADJACENT) {
-        const uint32_t c = slot ^ (line & 7);
+        const uint32_t c = Shape::swap(line, slot);
         chunk_k[n] = c * E;
         offset[n] = line < high ? (uint32_t)(line * ld * sizeof(T)) + c * 16 : kOutside;
       } else {
-        const uint32_t c = sizeof(T) == 2 ? slot ^ (4 * (line & 3)) : slot;
+        const uint32_t c = Shape::swap(line, slot);
         offset[n] = c * E < high ? (uint32_t)(line * ld * sizeof(T)) + c * 16 : kOutside;
       }
     }
@@ -620,23 +624,260 @@ __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a
   }
 }
 
-// The parts of a K that was split, in order, then the epilogue.
-template <typename T>
+// The parts of a K that was split, then the epilogue.  GROUPS threads share an output quad:
+// each adds a run of parts, in order, and the first one adds the runs, in order.
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, uint32_t split,
                                                         long long I, long long J, Epilogue e) {
+  constexpr int kWide = kThreads / GROUPS;
+  __shared__ f32x4 s_sum[GROUPS][kWide];
+  const uint32_t x = threadIdx.x % kWide, group = threadIdx.x / kWide;
   const long long quads = (J + 3) / 4;
-  const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-  if (id >= I * quads) return;
+  const long long id = (long long)blockIdx.x * kWide + x;
+  const bool on = id < I * quads;
   const long long i = id / quads, j = (id - i * quads) * 4;
   const int n = (int)min(4ll, J - j);
+  const uint32_t run = (split + GROUPS - 1) / GROUPS;
+  const uint32_t first = min(group * run, split), stop = min(first + run, split);
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  const float* p = partial + i * J + j;
-  for (uint32_t s = 0; s < split; ++s, p += I * J) {
+  if (on) {
+    const float* p = partial + ((long long)first * I + i) * J + j;
+#pragma unroll 8
+    for (uint32_t s = first; s < stop; ++s, p += I * J) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < n) sum[q] += p[q];
+      for (int q = 0; q < 4; ++q) sum[q] += p[min(q, n - 1)];
+    }
   }
-  finish<T>(e, i, j, n, sum);
+  if constexpr (GROUPS > 1) {
+    s_sum[group][x] = sum;
+    __syncthreads();
+    if (group) return;
+#pragma unroll
+    for (int g = 1; g < GROUPS; ++g) sum += s_sum[g][x];
+  }
+  if (on) finish<T>(e, i, j, n, sum);
+}
+
+// ------------------------------------------------------------------------ many rows, few columns
+//
+// J <= 32 NJ, B small enough to stay in LDS: a workgroup lays B out in fragment order once and
+// its waves stream rows of A, 32 at a time, from memory right into the matrix units' operand
+// registers, the next kChunk steps ahead of the products.  Nothing but A's rows and the
+// result moves, at any alignment.
+constexpr int kChunk = 8;  // steps in flight per wave: 32 rows x 256 bytes
+
+template <typename T>
+struct ThinArgs {
+  TileArgs t;
+  uint32_t blocks, steps;  // row blocks of 32; steps of k
+  int b_layout;
+};
+
+template <typename T, int NJ>
+__global__ __launch_bounds__(kThreads) void thin_kernel(const ThinArgs<T> args) {
+  constexpr int E = 16 / sizeof(T), kStep = 2 * E;
+  constexpr int kPair = NJ < 2 ? 1 : 2;  // column blocks that pass through LDS together
+  constexpr uint32_t kQuads = kPair * 8;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const TileArgs& a = args.t;
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const T* pb = (const T*)a.b;
+  for (uint32_t q = threadIdx.x; q < NJ * args.steps * 64; q += kThreads) {
+    const uint32_t l = q % 64, s = q / 64 % args.steps, jb = q / 64 / args.steps;
+    const long long j = jb * 32 + l % 32, k = (long long)s * kStep + l / 32 * E;
+    u32x4 v = {0, 0, 0, 0};
+    if (j < a.J) {
+      if (args.b_layout == K_ADJACENT) {
+        v = load16<T>(pb + j * a.ldb + k, a.K - k);
+      } else {
+        T r[E];
+#pragma unroll
+        for (int n = 0; n < E; ++n) r[n] = k + n < a.K ? pb[(k + n) * a.ldb + j] : (T)0.f;
+        __builtin_memcpy(&v, r, 16);
+      }
+    }
+    *reinterpret_cast<u32x4*>(lds + (size_t)q * 16) = v;
+  }
+  __syncthreads();
+  char* turn = lds + (size_t)NJ * args.steps * 1024 + wave * (kPair * 4096);
+
+  const uint32_t chunks = (args.steps + kChunk - 1) / kChunk;
+  const uint32_t stride = gridDim.x * (kThreads / 64);
+  uint32_t block = blockIdx.x * (kThreads / 64) + wave, chunk = 0;
+  if (block >= args.blocks) return;
+  f32x16 acc[NJ];
+#pragma unroll
+  for (int y = 0; y < NJ; ++y)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[y][r] = 0.f;
+
+  auto fetch = [&](u32x4(&f)[kChunk], uint32_t blk, uint32_t chk) {
+    const long long i = min((long long)blk * 32 + lane % 32, a.I - 1);
+    const T* p = (const T*)a.a + i * a.lda + (lane / 32 * E + chk * (kChunk * kStep));
+    const long long left = a.K - (long long)chk * (kChunk * kStep);
+    if (left >= kChunk * kStep) {
+#pragma unroll
+      for (int s = 0; s < kChunk; ++s) f[s] = load16<T>(p + s * kStep, E);
+    } else {
+      const long long mine = left - lane / 32 * E;
+#pragma unroll
+      for (int s = 0; s < kChunk; ++s) {
+        if (s * kStep < left) f[s] = load16<T>(p + s * kStep, mine - s * kStep);
+      }
+    }
+  };
+  auto use = [&](const u32x4(&f)[kChunk], uint32_t blk, uint32_t chk) {
+    const uint32_t s0 = chk * kChunk;
+    const char* pf = lds + (size_t)(s0 * 64 + lane) * 16;
+#pragma unroll
+    for (int s = 0; s < kChunk; ++s) {
+      if (s0 + s < args.steps) {
+#pragma unroll
+        for (int y = 0; y < NJ; ++y) {
+          const u32x4 fb =
+              *reinterpret_cast<const u32x4*>(pf + ((size_t)y * args.steps + s) * 1024);
+          acc[y] = Mfma<T>::run(fb, f[s], acc[y]);
+        }
+      }
+    }
+    if (chk + 1 < chunks) return;
+    const long long left = a.I - (long long)blk * 32;
+    const uint32_t high = (uint32_t)min(32ll, left);
+#pragma unroll
+    for (int y0 = 0; y0 < NJ; y0 += kPair) {
+#pragma unroll
+      for (int y = 0; y < kPair; ++y) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t i = lane % 32, q = y * 8 + 2 * g + lane / 32;
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            v[r] = acc[y0 + y][4 * g + r];
+            acc[y0 + y][4 * g + r] = 0.f;
+          }
+          *reinterpret_cast<f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16) = v;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      const uint32_t q = lane % kQuads;
+      const long long j = y0 * 32 + q * 4;
+      const int n = (int)min(4ll, a.J - j);
+      if (n > 0) {
+#pragma unroll 1
+        for (uint32_t i = lane / kQuads; i < high; i += 64 / kQuads) {
+          const f32x4 v =
+              *reinterpret_cast<const f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16);
+          finish<T>(a.e, (long long)blk * 32 + i, j, n, v);
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+  };
+
+  u32x4 one[kChunk], two[kChunk];
+  fetch(one, block, chunk);
+  while (true) {
+    uint32_t block2 = block, chunk2 = chunk + 1;
+    if (chunk2 == chunks) chunk2 = 0, block2 += stride;
+    if (block2 < args.blocks) fetch(two, block2, chunk2);
+    use(one, block, chunk);
+    if (block2 >= args.blocks) break;
+    block = block2, chunk = chunk2 + 1;
+    if (chunk == chunks) chunk = 0, block += stride;
+    if (block < args.blocks) fetch(one, block, chunk);
+    use(two, block2, chunk2);
+    if (block >= args.blocks) break;
+  }
+}
+
+// ------------------------------------------------------------------------ few rows, any weight
+//
+// I <= 16 NI: what counts is reading B, once and by the whole card.  A workgroup takes 16 rows
+// of B; its waves share out k, each streaming its part of the 16 rows into the matrix units'
+// operands, and their sums meet in LDS.  One launch, no scratch memory.
+template <typename T>
+struct SmallMfma;
+template <>
+struct SmallMfma<float> {
+  static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0,
+                                               0, 0);
+    return c;
+  }
+};
+template <>
+struct SmallMfma<_Float16> {
+  static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct SmallMfma<__bf16> {
+  static __device__ __forceinline__ f32x4 run(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+
+constexpr int kFewWaves = 16;
+
+template <typename T, int NI>
+__global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const TileArgs a) {
+  constexpr int E = 16 / sizeof(T), kStep = 4 * E, kAhead = 4;
+  __shared__ f32x4 s_sum[kFewWaves][NI][64];
+  const uint32_t lane = threadIdx.x % 64;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t waves = blockDim.x / 64;
+  const long long j0 = (long long)blockIdx.x * 16;
+  const long long row = min(j0 + lane % 16, a.J - 1);
+  const T* pb = (const T*)a.b + row * a.ldb + lane / 16 * E;
+  const T* pa[NI];
+#pragma unroll
+  for (int x = 0; x < NI; ++x)
+    pa[x] = (const T*)a.a + min((long long)x * 16 + lane % 16, a.I - 1) * a.lda + lane / 16 * E;
+  const uint32_t steps = (uint32_t)((a.K + kStep - 1) / kStep);
+  f32x4 acc[NI];
+#pragma unroll
+  for (int x = 0; x < NI; ++x) acc[x] = {0.f, 0.f, 0.f, 0.f};
+  // waves take neighbouring steps: together they read whole rows
+  for (uint32_t s0 = wave; s0 < steps; s0 += waves * kAhead) {
+    u32x4 fb[kAhead], fa[kAhead][NI];
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      const uint32_t s = s0 + n * waves;
+      if (s < steps) {
+        const long long k = (long long)s * kStep, left = a.K - k - lane / 16 * E;
+        fb[n] = load16<T>(pb + k, left);
+#pragma unroll
+        for (int x = 0; x < NI; ++x) fa[n][x] = load16<T>(pa[x] + k, left);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) {
+      if (s0 + n * waves < steps) {
+#pragma unroll
+        for (int x = 0; x < NI; ++x) acc[x] = SmallMfma<T>::run(fb[n], fa[n][x], acc[x]);
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < NI; ++x) s_sum[wave][x][lane] = acc[x];
+  __syncthreads();
+  if (wave >= NI) return;
+  f32x4 sum = s_sum[0][wave][lane];
+  for (uint32_t w = 1; w < waves; ++w) sum += s_sum[w][wave][lane];
+  // lane: row 16 x + lane % 16 of A, 4 neighbouring rows of B
+  const long long i = wave * 16 + lane % 16, j = j0 + lane / 16 * 4;
+  if (i < a.I && j < a.J) finish<T>(a.e, i, j, (int)min(4ll, a.J - j), sum);
 }
 
 // --------------------------------------------------------------- gradient of z, bias gradient
@@ -716,15 +957,36 @@ __global__ __launch_bounds__(kThreads) void grad_bias_kernel(const float* sums, 
 
 constexpr int kUnits = 256;  // compute units to fill
 
+// Which kernel runs a product, by sizes and alignment alone:
+//   FEW    few rows, both operands with k adjacent (forward)
+//   THIN   many rows, few columns, A with k adjacent (forward, dx)
+//   TILE   anything;  STREAM_*  both operands aligned, by the tile's rows x columns
+enum Kernel { FEW, THIN, TILE, STREAM_32x256, STREAM_128, STREAM_256 };
+
 struct Product {
+  Kernel kernel;
   uint32_t ti, tj, split;
   long long k_part;
-  int edge;     // rows and columns of a tile
-  bool direct;  // stream_kernel (both operands aligned) or tile_kernel
   long long bytes(long long I, long long J) const {
     return split > 1 ? (long long)split * I * J * 4 : 0;
   }
 };
+
+constexpr int kFewRows = 64;
+constexpr int kThinColumns = 256;
+constexpr long long kThinRows = 16384;
+constexpr uint32_t kThinLds = 81920;  // half a compute unit's: two workgroups share one
+
+uint32_t thin_blocks(long long J) {  // 32-column blocks: 1, 2, 4 or 8
+  return J <= 32 ? 1 : J <= 64 ? 2 : J <= 128 ? 4 : 8;
+}
+
+uint32_t thin_lds(long long J, long long K, int size) {
+  const uint32_t nj = thin_blocks(J);
+  const long long steps = (K * size + 31) / 32;
+  const long long bytes = nj * steps * 1024 + 4 * (nj < 2 ? 1 : 2) * 4096;
+  return bytes > kThinLds ? 0 : (uint32_t)bytes;
+}
 
 // An operand that stream_kernel can take: every 16-byte chunk aligned and not across an end,
 // a tile's offsets below 2^31.
@@ -737,16 +999,33 @@ bool streamable(const void* p, long long ld, int layout, long long rows, long lo
 
 // K is split where the tiles alone leave compute units idle, into parts of at least four
 // steps (512 bytes of k).
-bool plan_product(long long I, long long J, long long K, int dtype, bool direct, Product* p) {
-  p->direct = direct;
-  p->edge = 128;
-  if (direct && dtype != TEMPO_DTYPE_F32 && (I + 255) / 256 * ((J + 255) / 256) >= kUnits)
-    p->edge = 256;
-  const long long ti = (I + p->edge - 1) / p->edge, tj = (J + p->edge - 1) / p->edge;
+bool plan_product(long long I, long long J, long long K, int al, int bl, int dtype, bool direct,
+                  Product* p) {
+  const int size = dtype == TEMPO_DTYPE_F32 ? 4 : 2;
+  p->split = 1;
+  p->k_part = K;
+  if (al == K_ADJACENT && bl == K_ADJACENT && I <= kFewRows) {
+    p->kernel = FEW;
+    return true;
+  }
+  if (al == K_ADJACENT && J <= kThinColumns && I >= kThinRows && thin_lds(J, K, size)) {
+    p->kernel = THIN;
+    return true;
+  }
+  long long high = 128, wide = 128;
+  p->kernel = direct ? STREAM_128 : TILE;
+  if (direct && al == ROW_ADJACENT && I <= 32) {
+    p->kernel = STREAM_32x256;
+    high = 32, wide = 256;
+  } else if (direct && size == 2 && (I + 255) / 256 * ((J + 255) / 256) >= kUnits) {
+    p->kernel = STREAM_256;
+    high = wide = 256;
+  }
+  const long long ti = (I + high - 1) / high, tj = (J + wide - 1) / wide;
   if (ti > 0x3fffffff / tj) return false;
   p->ti = (uint32_t)ti;
   p->tj = (uint32_t)tj;
-  const long long depth = dtype == TEMPO_DTYPE_F32 ? 32 : 64;
+  const long long depth = 128 / size;
   const long long steps = (K + depth - 1) / depth;
   long long split = 2 * kUnits / (ti * tj);
   if (split > steps / 4) split = steps / 4;
@@ -758,13 +1037,53 @@ bool plan_product(long long I, long long J, long long K, int dtype, bool direct,
 }
 
 // Scratch memory is planned from sizes alone: either kernel may run in the end.
-bool product_bytes(long long I, long long J, long long K, int dtype, long long* bytes) {
+bool product_bytes(long long I, long long J, long long K, int al, int bl, int dtype,
+                   long long* bytes) {
   Product a, b;
-  if (!plan_product(I, J, K, dtype, false, &a) || !plan_product(I, J, K, dtype, true, &b))
+  if (!plan_product(I, J, K, al, bl, dtype, false, &a) ||
+      !plan_product(I, J, K, al, bl, dtype, true, &b))
     return false;
   const long long x = a.bytes(I, J), y = b.bytes(I, J);
   *bytes = x > y ? x : y;
   return true;
+}
+
+template <typename T>
+int run_few(const TileArgs& t, hipStream_t stream) {
+  const dim3 grid((unsigned)((t.J + 15) / 16));
+  const long long steps = (t.K * (long long)sizeof(T) + 63) / 64;
+  const dim3 block((unsigned)(steps < kFewWaves ? (steps < 4 ? 4 : steps) : kFewWaves) * 64);
+  if (t.I <= 16)
+    hipLaunchKernelGGL((few_kernel<T, 1>), grid, block, 0, stream, t);
+  else if (t.I <= 32)
+    hipLaunchKernelGGL((few_kernel<T, 2>), grid, block, 0, stream, t);
+  else
+    hipLaunchKernelGGL((few_kernel<T, 4>), grid, block, 0, stream, t);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int NJ>
+void launch_thin(const ThinArgs<T>& a, uint32_t lds, hipStream_t stream) {
+  const uint32_t groups = (a.blocks + 3) / 4;
+  const dim3 grid(groups < 2 * kUnits ? groups : 2 * kUnits);
+  hipLaunchKernelGGL((thin_kernel<T, NJ>), grid, dim3(kThreads), lds, stream, a);
+}
+
+template <typename T>
+int run_thin(const TileArgs& t, int b_layout, hipStream_t stream) {
+  ThinArgs<T> a = {};
+  a.t = t;
+  a.blocks = (uint32_t)((t.I + 31) / 32);
+  a.steps = (uint32_t)((t.K * (long long)sizeof(T) + 31) / 32);
+  a.b_layout = b_layout;
+  const uint32_t lds = thin_lds(t.J, t.K, sizeof(T));
+  switch (thin_blocks(t.J)) {
+    case 1: launch_thin<T, 1>(a, lds, stream); break;
+    case 2: launch_thin<T, 2>(a, lds, stream); break;
+    case 4: launch_thin<T, 4>(a, lds, stream); break;
+    default: launch_thin<T, 8>(a, lds, stream); break;
+  }
+  return (int)hipGetLastError();
 }
 
 template <typename T, int AL, int BL>
@@ -773,7 +1092,7 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
                 hipStream_t stream) {
   constexpr int dtype = sizeof(T) == 4 ? TEMPO_DTYPE_F32 : TEMPO_DTYPE_F16;
   Product p;
-  plan_product(I, J, K, dtype,
+  plan_product(I, J, K, AL, BL, dtype,
                streamable(a, lda, AL, I, K, sizeof(T)) && streamable(b, ldb, BL, J, K, sizeof(T)),
                &p);
   TileArgs t = {};
@@ -782,18 +1101,32 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
   t.e = e;
   t.e.partial = p.split > 1 ? scratch : nullptr;
   const dim3 grid(p.ti * p.tj, p.split);
-  if (!p.direct) {
+  if constexpr (AL == K_ADJACENT && BL == K_ADJACENT) {
+    if (p.kernel == FEW) return run_few<T>(t, stream);
+  }
+  if constexpr (AL == K_ADJACENT) {
+    if (p.kernel == THIN) return run_thin<T>(t, BL, stream);
+  }
+  if (p.kernel == TILE)
     hipLaunchKernelGGL((tile_kernel<T, AL, BL>), grid, dim3(kThreads), 0, stream, t);
-  } else if (p.edge == 128) {
+  if (p.kernel == STREAM_128)
     hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2>), grid, dim3(256), 0, stream, t);
-  } else {
-    if constexpr (sizeof(T) == 2)
+  if constexpr (AL == ROW_ADJACENT) {
+    if (p.kernel == STREAM_32x256)
+      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 1, 4, 1, 2>), grid, dim3(256), 0, stream, t);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (p.kernel == STREAM_256)
       hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 4, 4, 2>), grid, dim3(512), 0, stream, t);
   }
   if (p.split > 1) {
     const long long quads = I * ((J + 3) / 4);
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((quads + kThreads - 1) / kThreads)),
-                       dim3(kThreads), 0, stream, scratch, p.split, I, J, e);
+    if (p.split >= 16)
+      hipLaunchKernelGGL((join_kernel<T, 16>), dim3((unsigned)((quads + 15) / 16)),
+                         dim3(kThreads), 0, stream, scratch, p.split, I, J, e);
+    else
+      hipLaunchKernelGGL((join_kernel<T, 1>), dim3((unsigned)((quads + kThreads - 1) / kThreads)),
+                         dim3(kThreads), 0, stream, scratch, p.split, I, J, e);
   }
   return (int)hipGetLastError();
 }
@@ -807,7 +1140,8 @@ long long up16(long long n) { return (n + 15) / 16 * 16; }
 
 bool plan_backward(long long M, int N, int K, int dtype, int act, BackwardPlan* p) {
   long long x, w;
-  if (!product_bytes(M, K, N, dtype, &x) || !product_bytes(N, K, M, dtype, &w)) return false;
+  if (!product_bytes(M, K, N, K_ADJACENT, ROW_ADJACENT, dtype, &x) ||
+      !product_bytes(N, K, M, ROW_ADJACENT, ROW_ADJACENT, dtype, &w)) return false;
   p->dz_bytes = act == NONE ? 0 : up16(M * N * (dtype == TEMPO_DTYPE_F32 ? 4 : 2));
   p->sum_bytes = up16((M + kRowsPerBlock - 1) / kRowsPerBlock * N * 4);
   p->scratch_bytes = up16(x > w ? x : w);
@@ -871,7 +1205,7 @@ long long tempo_linear_workspace(long long M, int N, int K, int dtype, int activ
     return plan_backward(M, N, K, dtype, activation, &p) ? p.total() : TEMPO_E_SIZE;
   }
   long long bytes;
-  return product_bytes(M, N, K, dtype, &bytes) ? bytes : TEMPO_E_SIZE;
+  return product_bytes(M, N, K, K_ADJACENT, K_ADJACENT, dtype, &bytes) ? bytes : TEMPO_E_SIZE;
 }
 
 int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw,
@@ -882,7 +1216,7 @@ int tempo_linear(const void* x, long long ldx, const void* weight, long long ldw
   const int rc = check_sizes(M, N, K, dtype, activation);
   if (rc != TEMPO_OK) return rc;
   long long need;
-  if (!product_bytes(M, N, K, dtype, &need)) return TEMPO_E_SIZE;
+  if (!product_bytes(M, N, K, K_ADJACENT, K_ADJACENT, dtype, &need)) return TEMPO_E_SIZE;
   if (ldx < 0 || ldw < 0 || ldr < 0 || (M > 1 && ldy < N)) return TEMPO_E_ARG;
   if (misaligned(x, dtype) || misaligned(weight, dtype) || misaligned(y, dtype) ||
       misaligned(bias, dtype) || misaligned(residual, dtype) || misaligned(pre, dtype))

@@ -81,6 +81,28 @@ def test_more_tiles_than_compute_units(shape, dtype, gpu_device):
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', [(16411, 256, 32), (16384, 256, 64), (16400, 321, 17),
+                                   (16385, 24, 40), (20001, 64, 100), (16411, 32, 256),
+                                   (16390, 520, 8), (16384, 1, 1), (16400, 130, 129)], ids=str)
+def test_many_rows_of_few_channels(shape, dtype, gpu_device):
+    M, K, N = shape
+    for i, act in enumerate(('none', ACTS[1 + (M + K + N) % 5])):
+        _check_grads(_make(M, K, N, dtype, gpu_device, seed=5 + i, bias=i == 0, residual=i == 1,
+                           grad=True), act, f'{act} ')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('M', [1, 15, 16, 17, 32, 33, 64, 65])
+def test_few_rows(M, dtype, gpu_device):
+    for K, N in ((1000, 300), (72, 33), (1029, 17), (4096, 16)):
+        t = _make(M, K, N, dtype, gpu_device, seed=7, residual=True)
+        import tempo_amd
+        ref = R.linear(t['x'], t['weight'], t['bias'], t['residual'], 'silu')
+        y = tempo_amd.fused_linear(t['x'], t['weight'], t['bias'], t['residual'], 'silu')
+        R.check(y, ref['y'], ref['y_tol'], f'y, {K} x {N}')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize('act', ACTS)
 def test_activations_over_their_range(act, dtype, gpu_device):
     """K = 1 and a weight of 1: z runs over the whole range, infinities at the ends."""

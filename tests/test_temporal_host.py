@@ -95,9 +95,9 @@ def test_linear_entry_points_reject_bad_arguments():
         assert call(x=P(18)) == -5 and call(weight=P(17), dtype=2) == -5
         assert call(M=1 << 32) == -4 and call(N=1 << 21) == -4 and call(K=1 << 21) == -4
         assert call(ldx=-1) == -5 and call(ldw=-1) == -5
-        assert call(ws=P(24), K=65536, bytes=1 << 40) == -5
-        assert call(K=65536, bytes=8, lddx=65536) == -4
-    assert forward(K=65536, ws=None) == -1
+        assert call(ws=P(24), K=65536, M=100, bytes=1 << 40) == -5
+        assert call(K=65536, M=100, bytes=8, lddx=65536) == -4
+    assert forward(K=65536, M=100, ws=None) == -1
     assert forward(ldy=15) == -5 and backward(lddx=63) == -5 and backward(ldg=-1) == -5
     for name in ('y', 'bias', 'residual', 'pre'):
         assert forward(**{name: P(18)}) == -5
