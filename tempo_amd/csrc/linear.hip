@@ -199,22 +199,25 @@ __device__ __forceinline__ u32x4 load16(const T* p, long long left) {
   return out;
 }
 
-// One operand's tile in LDS: ROWS rows x 128 bytes of k.  16-byte chunks are permuted within
-// their row so that the reads below hit every bank equally:
-//   K_ADJACENT    [row][k]: chunk c of row r at c ^ (r % 8)
+// One operand's tile in LDS: ROWS rows x BYTES of k.  16-byte chunks are permuted within their
+// row so that the 16 lanes which the LDS serves at a time hit every bank once:
+//   K_ADJACENT    [row][k], 128 bytes: chunk c of row r at c ^ (r / 2 % 8), for two rows are all
+//                 banks (c ^ (r % 8): half of the LDS's cycles were conflicts);  64 bytes: four
+//                 rows are, c ^ (r / 4 % 4)
 //   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4) (32 rows: as it is, four
 //                 lines are all banks already);  fp32: as it is
-template <typename T, int LAYOUT, int ROWS>
+template <typename T, int LAYOUT, int ROWS, int BYTES = 128>
 struct Tile {
   static constexpr int E = 16 / sizeof(T);
-  static constexpr int kDepth = 128 / sizeof(T);
-  static constexpr int kLine = LAYOUT == K_ADJACENT ? 8 : ROWS / E;  // chunks per line
-  static constexpr int kBytes = ROWS * 128;
+  static constexpr int kDepth = BYTES / sizeof(T);
+  static constexpr int kSteps = BYTES / 32;
+  static constexpr int kLine = LAYOUT == K_ADJACENT ? BYTES / 16 : ROWS / E;  // chunks per line
+  static constexpr int kBytes = ROWS * BYTES;
   static constexpr int kPerThread = ROWS * 8 / kThreads;
 
   static __device__ __forceinline__ uint32_t swap(uint32_t line, uint32_t c) {
     if constexpr (LAYOUT == K_ADJACENT)
-      return c ^ (line & 7);
+      return BYTES == 128 ? c ^ (line / 2 & 7) : c ^ (line / 4 & 3);
     else if constexpr (sizeof(T) == 2 && ROWS >= 128)
       return c ^ (4 * (line & 3));
     else
@@ -292,47 +295,132 @@ __device__ __forceinline__ void tile_of(uint32_t id, uint32_t ti, uint32_t tj, u
   *j = in / high;
 }
 
-template <typename T>
-__device__ __forceinline__ void finish(const Epilogue& e, long long i, long long j, int n,
-                                       f32x4 acc) {
+template <bool FULL, int ROWS>
+__device__ __forceinline__ void activate_rows(f32x4 (&z)[ROWS], int act) {
+  switch (act) {  // one branch for all of them
+#define TEMPO_EACH(name)                                                              \
+  case name:                                                                          \
+    _Pragma("unroll") for (int r = 0; r < ROWS; ++r) _Pragma("unroll") for (int q = 0; q < 4; ++q) \
+        z[r][q] = activate<FULL>(z[r][q], name);                                      \
+    break;
+    TEMPO_EACH(RELU)
+    TEMPO_EACH(SILU)
+    TEMPO_EACH(GELU)
+    TEMPO_EACH(SIGMOID)
+    TEMPO_EACH(TANH)
+#undef TEMPO_EACH
+    default: break;
+  }
+}
+
+// The epilogue of ROWS quads of one column group, rows `apart` from each other, those from
+// `stop` on left out; n of the 4 columns are inside the matrix.  The residuals of all of them
+// are on their way before the first one is needed: one at a time, their latency took longer
+// than the products (256 x 256 tiles of 16384 x 4096 x 4096: 590 us against 415).
+template <typename T, int ROWS>
+__device__ __forceinline__ void finish(const Epilogue& e, long long i, uint32_t apart,
+                                       long long stop, long long j, int n, f32x4 (&z)[ROWS]) {
   constexpr bool FULL = sizeof(T) == 4;
   typedef typename Pack<T, 4>::type V4;
-  float z[4], y[4];
+  V4 residual[ROWS];
+  if (e.residual) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) z[q] = acc[q];
-  if (n == 4) {
-    if (e.bias) {
-      const V4 b = *reinterpret_cast<const V4*>((const T*)e.bias + j);
+    for (int r = 0; r < ROWS; ++r) {
+      const T* p = (const T*)e.residual + min(i + r * apart, stop - 1) * e.ldr + j;
+      if (n == 4) {
+        residual[r] = *reinterpret_cast<const V4*>(p);
+      } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) z[q] += (float)b[q];
+        for (int q = 0; q < 4; ++q) residual[r][q] = q < n ? p[q] : (T)0.f;
+      }
     }
-    if (e.pre) {
-      V4 p;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) p[q] = keep_sign<T>(z[q]);
-      *reinterpret_cast<V4*>((T*)e.pre + i * e.ldp + j) = p;
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q) y[q] = activate<FULL>(z[q], e.act);
-    if (e.residual) {
-      const V4 r = *reinterpret_cast<const V4*>((const T*)e.residual + i * e.ldr + j);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) y[q] += (float)r[q];
-    }
-    V4 o;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) o[q] = (T)y[q];
-    *reinterpret_cast<V4*>((T*)e.out + i * e.ldo + j) = o;
-  } else {
+  }
+  if (e.bias) {
+    const T* p = (const T*)e.bias + j;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (q < n) {
-        if (e.bias) z[q] += (float)((const T*)e.bias)[j + q];
-        if (e.pre) ((T*)e.pre)[i * e.ldp + j + q] = keep_sign<T>(z[q]);
-        float v = activate<FULL>(z[q], e.act);
-        if (e.residual) v += (float)((const T*)e.residual)[i * e.ldr + j + q];
-        ((T*)e.out)[i * e.ldo + j + q] = (T)v;
+      const float b = (float)p[min(q, n - 1)];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) z[r][q] += b;
+    }
+  }
+  if (e.pre) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      if (i + r * apart >= stop) continue;
+      T* p = (T*)e.pre + (i + r * apart) * e.ldp + j;
+      V4 kept;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) kept[q] = keep_sign<T>(z[r][q]);
+      if (n == 4) {
+        *reinterpret_cast<V4*>(p) = kept;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < n) p[q] = kept[q];
       }
+    }
+  }
+  activate_rows<FULL, ROWS>(z, e.act);
+  if (e.residual) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) z[r][q] += (float)residual[r][q];
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    if (i + r * apart >= stop) continue;
+    T* p = (T*)e.out + (i + r * apart) * e.ldo + j;
+    V4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o[q] = (T)z[r][q];
+    if (n == 4) {
+      *reinterpret_cast<V4*>(p) = o;
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (q < n) p[q] = o[q];
+    }
+  }
+}
+
+constexpr int kTogether = 4;  // rows of an epilogue that are under way at a time
+
+// A slab of sums in LDS (row i, 16-byte chunk c at c ^ (i % 32)) to memory: rows row0 .. row0 +
+// high - 1 of C, threads side by side along a row.
+template <typename T, uint32_t QUADS, uint32_t THREADS>
+__device__ __forceinline__ void write_slab(const TileArgs& a, const char* lds, long long row0,
+                                           uint32_t high, long long j0) {
+  const uint32_t c = threadIdx.x % QUADS;
+  constexpr uint32_t kApart = THREADS / QUADS;
+  const long long j = j0 + c * 4;
+  if (j >= a.J) return;
+  const int n = (int)min(4ll, a.J - j);
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x / QUADS; i < high; i += kTogether * kApart) {
+    f32x4 v[kTogether];
+#pragma unroll
+    for (int r = 0; r < kTogether; ++r) {
+      const uint32_t row = min(i + r * kApart, high - 1);
+      v[r] = *reinterpret_cast<const f32x4*>(lds + (row * QUADS + (c ^ (row & 31))) * 16);
+    }
+    if (a.e.partial) {
+#pragma unroll
+      for (int r = 0; r < kTogether; ++r) {
+        if (i + r * kApart >= high) continue;
+        float* p = a.e.partial +
+                   ((long long)blockIdx.y * a.I + row0 + i + r * kApart) * a.J + j;
+        if (n == 4) {
+          *reinterpret_cast<Pack<float, 4>::type*>(p) = v[r];
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (q < n) p[q] = v[r][q];
+        }
+      }
+    } else {
+      finish<T, kTogether>(a.e, row0 + i, kApart, row0 + high, j, n, v);
     }
   }
 }
@@ -413,23 +501,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
     }
   }
   __syncthreads();
-  const uint32_t c = threadIdx.x % 32;
-  const long long j = j0 + c * 4;
-  if (j >= a.J) return;
-  const int n = (int)min(4ll, a.J - j);
-  const uint32_t high = (uint32_t)min(128ll, a.I - i0);
-#pragma unroll 1
-  for (uint32_t i = threadIdx.x / 32; i < high; i += kThreads / 32) {
-    const f32x4 v = *reinterpret_cast<const f32x4*>(lc + (i * 32 + (c ^ (i & 31))) * 16);
-    if (a.e.partial) {
-      float* p = a.e.partial + ((long long)blockIdx.y * a.I + i0 + i) * a.J + j;
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (q < n) p[q] = v[q];
-    } else {
-      finish<T>(a.e, i0 + i, j, n, v);
-    }
-  }
+  write_slab<T, 32, kThreads>(a, lc, i0, (uint32_t)min(128ll, a.I - i0), j0);
 }
 
 // ---------------------------------------------------- tile kernel on aligned operands
@@ -461,11 +533,12 @@ __device__ __forceinline__ void chunks_to_lds(uint32_t lds, uint32_t offset, u32
 }
 
 // One operand's way to LDS: kLoads instructions per wave and step
-template <typename T, int LAYOUT, int ROWS, int WAVES>
+template <typename T, int LAYOUT, int ROWS, int BYTES, int WAVES>
 struct Stream {
-  typedef Tile<T, LAYOUT, ROWS> Shape;
+  typedef Tile<T, LAYOUT, ROWS, BYTES> Shape;
   static constexpr int E = Shape::E;
-  static constexpr int kLoads = ROWS * 8 / (WAVES * 64);
+  static constexpr int kLoads = Shape::kBytes / (WAVES * 1024);
+  static_assert(kLoads * WAVES * 1024 == Shape::kBytes, "whole instructions");
   const T* base;
   long long ld;
   uint32_t offset[kLoads], chunk_k[kLoads];
@@ -499,50 +572,62 @@ struct Stream {
     }
   }
 
-  // the step's k: k .. k + kDepth - 1, those from K on are zeros
-  __device__ __forceinline__ void load(uint32_t lds, long long k, long long K,
-                                       uint32_t wave) const {
+  // One stage: k .. k + kDepth - 1; what lies at or beyond K becomes zeros, all of it where
+  // k >= K, so that every step issues the same loads and can count them.
+  struct Stage {
+    u32x4 buffer;
+    uint32_t at, left, lds;
+  };
+  __device__ __forceinline__ Stage stage(uint32_t lds, uint32_t k, uint32_t K) const {
+    Stage s;
+    s.lds = lds;
+    s.left = k < K ? K - k : 0;
     if constexpr (LAYOUT == K_ADJACENT) {
-      const u32x4 buffer = buffer_of(base, extent);
-      const uint32_t at = (uint32_t)(k * sizeof(T));
-      const bool whole = k + Shape::kDepth <= K;
-      const uint32_t left = (uint32_t)(K - k);
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n) {
-        const uint32_t o = whole || chunk_k[n] < left ? offset[n] : kOutside;
-        chunks_to_lds(lds + (n * WAVES + wave) * 1024, o, buffer, at);
-      }
+      s.buffer = buffer_of(base, extent);
+      s.at = __builtin_amdgcn_readfirstlane(s.left ? (uint32_t)(k * sizeof(T)) : 0u);
     } else {
-      const uint32_t lines = (uint32_t)min((long long)Shape::kDepth, K - k);
-      const u32x4 buffer =
-          buffer_of(base + k * ld, (uint32_t)(((lines - 1) * ld + rows) * sizeof(T)));
-#pragma unroll
-      for (int n = 0; n < kLoads; ++n)
-        chunks_to_lds(lds + (n * WAVES + wave) * 1024, offset[n], buffer, 0);
+      const uint32_t lines = min((uint32_t)Shape::kDepth, s.left);
+      s.buffer = buffer_of(base + (s.left ? k * ld : 0),
+                           lines ? (uint32_t)(((lines - 1) * ld + rows) * sizeof(T)) : 0u);
+      s.at = 0;
     }
+    return s;
+  }
+  __device__ __forceinline__ void load(const Stage& s, int n, uint32_t wave) const {
+    const uint32_t o =
+        LAYOUT == ROW_ADJACENT || chunk_k[n] < s.left ? offset[n] : kOutside;
+    chunks_to_lds(s.lds + (n * WAVES + wave) * 1024, o, s.buffer, s.at);
   }
 };
 
-// WI x WJ waves of XI x XJ blocks of 32 x 32
-template <typename T, int AL, int BL, int WI, int WJ, int XI, int XJ>
+template <int N>
+__device__ __forceinline__ void wait_loads() {  // until at most N of the wave's loads are under way
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// WI x WJ waves of XI x XJ blocks of 32 x 32; STAGES tiles of BYTES of k in LDS, of which one
+// is read while the others arrive.
+template <typename T, int AL, int BL, int WI, int WJ, int XI, int XJ, int BYTES, int STAGES>
 __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a) {
   constexpr int kWaves = WI * WJ, kRows = WI * XI * 32, kCols = WJ * XJ * 32;
-  typedef Tile<T, AL, kRows> TA;
-  typedef Tile<T, BL, kCols> TB;
+  typedef Tile<T, AL, kRows, BYTES> TA;
+  typedef Tile<T, BL, kCols, BYTES> TB;
   constexpr int kStage = TA::kBytes + TB::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(16))) char lds[STAGES * kStage];
   uint32_t i_tile, j_tile;
   tile_of(blockIdx.x, a.ti, a.tj, &i_tile, &j_tile);
   const long long i0 = (long long)i_tile * kRows, j0 = (long long)j_tile * kCols;
   const uint32_t lane = threadIdx.x % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const uint32_t wi = wave / WJ * XI * 32, wj = wave % WJ * XJ * 32;
-  const long long k_begin = blockIdx.y * a.k_part;
-  const long long k_end = min(a.K, k_begin + a.k_part);
+  const uint32_t k_begin = blockIdx.y * (uint32_t)a.k_part;
+  const uint32_t k_end = min((uint32_t)a.K, k_begin + (uint32_t)a.k_part);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
-  const Stream<T, AL, kRows, kWaves> sa(a.a, a.lda, i0, a.I, a.K, wave, lane);
-  const Stream<T, BL, kCols, kWaves> sb(a.b, a.ldb, j0, a.J, a.K, wave, lane);
+  typedef Stream<T, AL, kRows, BYTES, kWaves> SA;
+  typedef Stream<T, BL, kCols, BYTES, kWaves> SB;
+  const SA sa(a.a, a.lda, i0, a.I, a.K, wave, lane);
+  const SB sb(a.b, a.ldb, j0, a.J, a.K, wave, lane);
 
   f32x16 acc[XI][XJ];
 #pragma unroll
@@ -552,39 +637,74 @@ __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
-  sa.load(lds0, k_begin, k_end, wave);
-  sb.load(lds0 + TA::kBytes, k_begin, k_end, wave);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  // Loads, LDS reads and products are dealt out evenly: issued in a burst behind the barrier,
+  // a stage's loads keep the compute unit's address path, and with it every wave, busy for
+  // longer than its products take.  A stage's loads are cut into kSteps portions: the first
+  // goes out behind the barrier that frees the stage's place, the others in the next round.
+  constexpr int kLoads = SA::kLoads + SB::kLoads;
+  constexpr int kPortion = (kLoads + TA::kSteps - 1) / TA::kSteps;
+  constexpr int kReads = XI + XJ;
+  u32x4 fa[2][XI], fb[2][XJ];  // one set feeds the products while the other one arrives
+  typename SA::Stage ga;
+  typename SB::Stage gb;
+  auto refill = [&](uint32_t place, uint32_t k) {
+    ga = sa.stage(lds0 + place, k, k_end);
+    gb = sb.stage(lds0 + place + TA::kBytes, k, k_end);
+  };
+  auto load = [&](int n) {
+    if (n < SA::kLoads) sa.load(ga, n, wave);
+    else if (n < kLoads) sb.load(gb, n - SA::kLoads, wave);
+  };
+  auto read = [&](int set, uint32_t place, int step, int n) {
+    if (n < XJ) fb[set][n] = TB::fragment(lds + place + TA::kBytes, wj + 32 * n, step, lane);
+    else fa[set][n - XJ] = TA::fragment(lds + place, wi + 32 * (n - XJ), step, lane);
+  };
+  // products of one set, reads of the other, one portion of loads
+  auto phase = [&](int set, uint32_t place, int step, int portion) {
+#pragma unroll
+    for (int x = 0; x < XI; ++x) {
+#pragma unroll
+      for (int n = x * kReads / XI; n < (x + 1) * kReads / XI; ++n) read(set ^ 1, place, step, n);
+#pragma unroll
+      for (int y = 0; y < XJ; ++y)
+        acc[x][y] = Mfma<T>::run(fb[set][y], fa[set][x], acc[x][y]);
+#pragma unroll
+      for (int n = x * kPortion / XI; n < (x + 1) * kPortion / XI; ++n)
+        load(portion * kPortion + n);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+#pragma unroll
+  for (int n = 0; n < STAGES; ++n) {
+    refill(n * kStage, k_begin + n * TA::kDepth);
+#pragma unroll
+    for (int l = 0; l < (n < STAGES - 1 ? kLoads : kPortion); ++l) load(l);
+  }
+  wait_loads<(STAGES - 2) * kLoads + kPortion>();
   __syncthreads();
   uint32_t now = 0;
-  for (long long k = k_begin; k < k_end; k += TA::kDepth, now ^= kStage) {
-    if (k + TA::kDepth < k_end) {  // into the half that everyone has left at the last barrier
-      sa.load(lds0 + (now ^ kStage), k + TA::kDepth, k_end, wave);
-      sb.load(lds0 + (now ^ kStage) + TA::kBytes, k + TA::kDepth, k_end, wave);
-    }
-    const char* la = lds + now;
-    const char* lb = la + TA::kBytes;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      u32x4 fa[XI], fb[XJ];
+  for (int n = 0; n < kReads; ++n) read(0, 0, 0, n);
+  for (uint32_t k = k_begin; k < k_end; k += TA::kDepth) {
+    const uint32_t next = now + kStage < STAGES * kStage ? now + kStage : 0;
 #pragma unroll
-      for (int x = 0; x < XI; ++x) fa[x] = TA::fragment(la, wi + 32 * x, s, lane);
-#pragma unroll
-      for (int y = 0; y < XJ; ++y) fb[y] = TB::fragment(lb, wj + 32 * y, s, lane);
-#pragma unroll
-      for (int x = 0; x < XI; ++x)
-#pragma unroll
-        for (int y = 0; y < XJ; ++y) acc[x][y] = Mfma<T>::run(fb[y], fa[x], acc[x][y]);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the next step's chunks are in LDS
+    for (int step = 0; step < TA::kSteps - 1; ++step) phase(step & 1, now, step + 1, step + 1);
+    // The next stage has arrived (the STAGES - 2 behind it may still be under way) and everyone
+    // has read this one: refill it, and begin on the next under the last products of this one.
+    wait_loads<(STAGES - 2) * kLoads>();
     __syncthreads();
+    refill(now, k + STAGES * TA::kDepth);
+    phase(1, next, 0, 0);
+    now = next;
   }
+  wait_loads<0>();  // zeros on their way to stages behind the end
+  __syncthreads();
 
   // sums through LDS as above, kSlab rows at a time
-  constexpr uint32_t kSlab = 2 * kStage / (kCols * 4), kQuads = kCols / 4;
-  const uint32_t c = threadIdx.x % kQuads;
-  const long long j = j0 + c * 4;
-  const int n = (int)min(4ll, a.J - j);
+  constexpr uint32_t kFit = STAGES * kStage / (kCols * 4) / (XI * 32) * (XI * 32);
+  constexpr uint32_t kSlab = kFit < kRows ? kFit : kRows, kQuads = kCols / 4;
+  static_assert(kSlab > 0, "a wave's rows fit in LDS");
 #pragma unroll
   for (uint32_t slab = 0; slab < kRows; slab += kSlab) {
     if (slab) __syncthreads();
@@ -607,20 +727,7 @@ __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a
     __syncthreads();
     const long long left = a.I - i0 - slab;
     const uint32_t high = left < 0 ? 0u : (uint32_t)min((long long)kSlab, left);
-    if (n > 0) {
-#pragma unroll 1
-      for (uint32_t i = threadIdx.x / kQuads; i < high; i += kWaves * 64 / kQuads) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(lds + (i * kQuads + (c ^ (i & 31))) * 16);
-        if (a.e.partial) {
-          float* p = a.e.partial + ((long long)blockIdx.y * a.I + i0 + slab + i) * a.J + j;
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (q < n) p[q] = v[q];
-        } else {
-          finish<T>(a.e, i0 + slab + i, j, n, v);
-        }
-      }
-    }
+    write_slab<T, kQuads, kWaves * 64>(a, lds, i0 + slab, high, j0);
   }
 }
 
@@ -655,7 +762,10 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, ui
 #pragma unroll
     for (int g = 1; g < GROUPS; ++g) sum += s_sum[g][x];
   }
-  if (on) finish<T>(e, i, j, n, sum);
+  if (on) {
+    f32x4 z[1] = {sum};
+    finish<T, 1>(e, i, 0, i + 1, j, n, z);
+  }
 }
 
 // ------------------------------------------------------------------------ many rows, few columns
@@ -767,11 +877,17 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(const ThinArgs<T> args) 
       const long long j = y0 * 32 + q * 4;
       const int n = (int)min(4ll, a.J - j);
       if (n > 0) {
+        constexpr uint32_t kApart = 64 / kQuads;
 #pragma unroll 1
-        for (uint32_t i = lane / kQuads; i < high; i += 64 / kQuads) {
-          const f32x4 v =
-              *reinterpret_cast<const f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16);
-          finish<T>(a.e, (long long)blk * 32 + i, j, n, v);
+        for (uint32_t i = lane / kQuads; i < high; i += kTogether * kApart) {
+          f32x4 v[kTogether];
+#pragma unroll
+          for (int r = 0; r < kTogether; ++r) {
+            const uint32_t row = i + r * kApart;  // < 32, the block's rows
+            v[r] = *reinterpret_cast<const f32x4*>(
+                turn + (row * kQuads + (q ^ (row % kQuads))) * 16);
+          }
+          finish<T, kTogether>(a.e, (long long)blk * 32 + i, kApart, a.I, j, n, v);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -877,7 +993,10 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const TileArgs a) {
   for (uint32_t w = 1; w < waves; ++w) sum += s_sum[w][wave][lane];
   // lane: row 16 x + lane % 16 of A, 4 neighbouring rows of B
   const long long i = wave * 16 + lane % 16, j = j0 + lane / 16 * 4;
-  if (i < a.I && j < a.J) finish<T>(a.e, i, j, (int)min(4ll, a.J - j), sum);
+  if (i < a.I && j < a.J) {
+    f32x4 z[1] = {sum};
+    finish<T, 1>(a.e, i, 0, i + 1, j, (int)min(4ll, a.J - j), z);
+  }
 }
 
 // --------------------------------------------------------------- gradient of z, bias gradient
@@ -1110,14 +1229,14 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
   if (p.kernel == TILE)
     hipLaunchKernelGGL((tile_kernel<T, AL, BL>), grid, dim3(kThreads), 0, stream, t);
   if (p.kernel == STREAM_128)
-    hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2>), grid, dim3(256), 0, stream, t);
+    hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2, 64, 4>), grid, dim3(256), 0, stream, t);
   if constexpr (AL == ROW_ADJACENT) {
     if (p.kernel == STREAM_32x256)
-      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 1, 4, 1, 2>), grid, dim3(256), 0, stream, t);
+      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 1, 4, 1, 2, 128, 2>), grid, dim3(256), 0, stream, t);
   }
   if constexpr (sizeof(T) == 2) {
     if (p.kernel == STREAM_256)
-      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 4, 4, 2>), grid, dim3(512), 0, stream, t);
+      hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 4, 4, 2, 64, 4>), grid, dim3(512), 0, stream, t);
   }
   if (p.split > 1) {
     const long long quads = I * ((J + 3) / 4);
