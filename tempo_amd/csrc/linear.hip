@@ -19,6 +19,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/tempo_unproject.h"
 
 namespace {
@@ -425,9 +427,110 @@ __device__ __forceinline__ void write_slab(const TileArgs& a, const char* lds, l
   }
 }
 
+// 16 bytes moved down by n elements, zeros from above
+template <typename T>
+__device__ __forceinline__ u32x4 shift_down(u32x4 r, uint32_t n) {
+  const uint32_t bits = n * 8 * sizeof(T);
+  uint64_t lo = (uint64_t)r[1] << 32 | r[0], hi = (uint64_t)r[3] << 32 | r[2];
+  if (bits >= 128) lo = hi = 0;
+  else if (bits >= 64) lo = hi >> (bits - 64), hi = 0;
+  else if (bits) lo = lo >> bits | hi << (64 - bits), hi >>= bits;
+  const u32x4 out = {(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  return out;
+}
+
+// One operand's way to LDS through registers, for rows at any alignment.  Every load is whole
+// and inside the operand, without a branch: a chunk across the end of its row is loaded so that
+// it ends there and moved down afterwards, rows and k beyond the end are loaded from the last
+// ones, k beyond the end then set to 0.  Needs 16 bytes in the adjacent direction.
+template <typename T, int LAYOUT>
+struct Gather {
+  typedef Tile<T, LAYOUT, 128> Shape;
+  static constexpr int E = Shape::E, kCount = Shape::kPerThread;
+  const T* at[kCount];
+  long long ld;
+  uint32_t first[kCount];  // K_ADJACENT: a chunk's first k in its step; ROW_ADJACENT: its line
+  uint32_t move[kCount];   // ROW_ADJACENT: elements
+  bool edge;               // ROW_ADJACENT: some chunk needs to be moved
+
+  __device__ __forceinline__ Gather(const void* p, long long ld_, long long row0, long long rows) {
+    ld = ld_;
+    edge = LAYOUT == ROW_ADJACENT && row0 + 128 > rows;
+#pragma unroll
+    for (int n = 0; n < kCount; ++n) {
+      const uint32_t q = n * kThreads + threadIdx.x;
+      const uint32_t line = q / Shape::kLine, c = q % Shape::kLine;
+      if constexpr (LAYOUT == K_ADJACENT) {
+        at[n] = (const T*)p + min(row0 + line, rows - 1) * ld;
+        first[n] = c * E;
+        move[n] = 0;
+      } else {
+        const long long row = row0 + c * E, inside = min(row, rows - E);
+        at[n] = (const T*)p + inside;
+        first[n] = line;
+        move[n] = (uint32_t)(row - inside);
+      }
+    }
+  }
+
+  __device__ __forceinline__ void fetch(uint32_t k0, uint32_t K, u32x4 (&r)[kCount]) const {
+    typedef typename Pack<T, E>::type Chunk;
+    if (k0 + Shape::kDepth <= K) {
+#pragma unroll
+      for (int n = 0; n < kCount; ++n) {
+        const T* p = LAYOUT == K_ADJACENT ? at[n] + (k0 + first[n])
+                                          : at[n] + (k0 + first[n]) * ld;
+        r[n] = __builtin_bit_cast(u32x4, *reinterpret_cast<const Chunk*>(p));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < kCount; ++n) {
+        const uint32_t k = k0 + first[n];
+        const T* p = LAYOUT == K_ADJACENT ? at[n] + min(k, K - E) : at[n] + min(k, K - 1) * ld;
+        r[n] = __builtin_bit_cast(u32x4, *reinterpret_cast<const Chunk*>(p));
+      }
+#pragma unroll
+      for (int n = 0; n < kCount; ++n) {
+        const uint32_t k = k0 + first[n];
+        if constexpr (LAYOUT == K_ADJACENT) {
+          r[n] = shift_down<T>(r[n], k - min(k, K - E));
+        } else if (k >= K) {
+          r[n] = u32x4{0, 0, 0, 0};
+        }
+      }
+    }
+  }
+
+  __device__ __forceinline__ void put(char* lds, u32x4 (&r)[kCount]) const {
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < kCount; ++n) r[n] = shift_down<T>(r[n], move[n]);
+    }
+    Shape::put(lds, r);
+  }
+};
+
+// The same for operands shorter than that, element by element
+template <typename T, int LAYOUT>
+struct TinyGather {
+  typedef Tile<T, LAYOUT, 128> Shape;
+  const T* p;
+  long long ld, row0, rows;
+  __device__ __forceinline__ TinyGather(const void* p_, long long ld_, long long row0_,
+                                        long long rows_)
+      : p((const T*)p_), ld(ld_), row0(row0_), rows(rows_) {}
+  __device__ __forceinline__ void fetch(uint32_t k0, uint32_t K,
+                                        u32x4 (&r)[Shape::kPerThread]) const {
+    Shape::fetch(p, ld, row0, rows, k0, K, r);
+  }
+  __device__ __forceinline__ void put(char* lds, u32x4 (&r)[Shape::kPerThread]) const {
+    Shape::put(lds, r);
+  }
+};
+
 // 128 x 128 of C per workgroup, 4 waves of 64 x 64; loads of the next 128 bytes of k fly under
 // the products of the present ones.
-template <typename T, int AL, int BL>
+template <typename T, int AL, int BL, bool TINY>
 __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
   typedef Tile<T, AL, 128> TA;
   typedef Tile<T, BL, 128> TB;
@@ -437,9 +540,12 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
   const long long i0 = (long long)i_tile * 128, j0 = (long long)j_tile * 128;
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const uint32_t wi = wave / 2 * 64, wj = wave % 2 * 64;
-  const long long k_begin = blockIdx.y * a.k_part;
-  const long long k_end = min(a.K, k_begin + a.k_part);
-  const T *pa = (const T*)a.a, *pb = (const T*)a.b;
+  const uint32_t k_begin = blockIdx.y * (uint32_t)a.k_part, K = (uint32_t)a.K;
+  const uint32_t k_end = min(K, k_begin + (uint32_t)a.k_part);
+  typedef typename std::conditional<TINY, TinyGather<T, AL>, Gather<T, AL>>::type GA;
+  typedef typename std::conditional<TINY, TinyGather<T, BL>, Gather<T, BL>>::type GB;
+  const GA ga(a.a, a.lda, i0, a.I);
+  const GB gb(a.b, a.ldb, j0, a.J);
 
   f32x16 acc[2][2];
 #pragma unroll
@@ -450,36 +556,43 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
   u32x4 ra[TA::kPerThread], rb[TB::kPerThread];
-  TA::fetch(pa, a.lda, i0, a.I, k_begin, k_end, ra);
-  TB::fetch(pb, a.ldb, j0, a.J, k_begin, k_end, rb);
-  TA::put(lds[0], ra);
-  TB::put(lds[0] + TA::kBytes, rb);
+  ga.fetch(k_begin, K, ra);
+  gb.fetch(k_begin, K, rb);
+  ga.put(lds[0], ra);
+  gb.put(lds[0] + TA::kBytes, rb);
   __syncthreads();
   int now = 0;
-  for (long long k = k_begin; k < k_end; k += TA::kDepth, now ^= 1) {
+  for (uint32_t k = k_begin; k < k_end; k += TA::kDepth, now ^= 1) {
     const bool more = k + TA::kDepth < k_end;
     if (more) {
-      TA::fetch(pa, a.lda, i0, a.I, k + TA::kDepth, k_end, ra);
-      TB::fetch(pb, a.ldb, j0, a.J, k + TA::kDepth, k_end, rb);
+      ga.fetch(k + TA::kDepth, K, ra);
+      gb.fetch(k + TA::kDepth, K, rb);
     }
     const char* la = lds[now];
     const char* lb = la + TA::kBytes;
+    u32x4 fa[2][2], fb[2][2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      fa[0][x] = TA::fragment(la, wi + 32 * x, 0, lane);
+      fb[0][x] = TB::fragment(lb, wj + 32 * x, 0, lane);
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      u32x4 fa[2], fb[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) fa[x] = TA::fragment(la, wi + 32 * x, s, lane);
-#pragma unroll
-      for (int y = 0; y < 2; ++y) fb[y] = TB::fragment(lb, wj + 32 * y, s, lane);
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
+      for (int x = 0; x < 2; ++x) {
+        if (s < 3) {  // the next step's operands arrive under this one's products
+          fa[s + 1 & 1][x] = TA::fragment(la, wi + 32 * x, s + 1, lane);
+          fb[s + 1 & 1][x] = TB::fragment(lb, wj + 32 * x, s + 1, lane);
+        }
 #pragma unroll
         for (int y = 0; y < 2; ++y)  // C^T: a lane holds 4 neighbouring j of one i
-          acc[x][y] = Mfma<T>::run(fb[y], fa[x], acc[x][y]);
+          acc[x][y] = Mfma<T>::run(fb[s & 1][y], fa[s & 1][x], acc[x][y]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (more) {
-      TA::put(lds[now ^ 1], ra);
-      TB::put(lds[now ^ 1] + TA::kBytes, rb);
+      ga.put(lds[now ^ 1], ra);
+      gb.put(lds[now ^ 1] + TA::kBytes, rb);
     }
     __syncthreads();
   }
@@ -1226,8 +1339,13 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
   if constexpr (AL == K_ADJACENT) {
     if (p.kernel == THIN) return run_thin<T>(t, BL, stream);
   }
-  if (p.kernel == TILE)
-    hipLaunchKernelGGL((tile_kernel<T, AL, BL>), grid, dim3(kThreads), 0, stream, t);
+  if (p.kernel == TILE) {
+    constexpr int e = 16 / sizeof(T);
+    if ((AL == K_ADJACENT ? K : I) < e || (BL == K_ADJACENT ? K : J) < e)
+      hipLaunchKernelGGL((tile_kernel<T, AL, BL, true>), grid, dim3(kThreads), 0, stream, t);
+    else
+      hipLaunchKernelGGL((tile_kernel<T, AL, BL, false>), grid, dim3(kThreads), 0, stream, t);
+  }
   if (p.kernel == STREAM_128)
     hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2, 64, 4>), grid, dim3(256), 0, stream, t);
   if constexpr (AL == ROW_ADJACENT) {
