@@ -1272,31 +1272,56 @@ def _float_tensor(t, name, dim, dtype=None, device=None):
     return t
 
 
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(what, dev, entry, *args):
+    """A C entry point on ``dev`` and its current stream (the last argument of all of them)."""
+    if dev.index == torch._C._cuda_getDevice():
+        rc = entry(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _raw_stream(dev))
+    if rc:
+        _lib.check(rc, what)
+
+
+def _workspace(bytes_, what, like):
+    """Scratch memory of one call.  From torch's allocator every time: its blocks follow the
+    stream (and, under capture, belong to the graph), so no two calls share one."""
+    if bytes_ < 0:
+        _lib.check(int(bytes_), what)
+    if not bytes_:
+        return None
+    return like.new_empty((bytes_ + 3) // 4, dtype=torch.float32)
+
+
 def _strided(t):
-    return _ptr(t), t.stride(0), t.stride(1)
+    return t.data_ptr(), t.stride(0), t.stride(1)
 
 
 def _like_time_order(t, channels):
     """Empty ``[B,T,channels]`` whose memory has time outermost where ``t``'s has."""
     B, T, _ = t.shape
     if B > 1 and T > 1 and t.stride(1) > t.stride(0):
-        return torch.empty(T, B, channels, dtype=t.dtype, device=t.device).transpose(0, 1)
-    return torch.empty(B, T, channels, dtype=t.dtype, device=t.device)
+        return t.new_empty((T, B, channels)).transpose(0, 1)
+    return t.new_empty((B, T, channels))
 
 
 def _recurrence_inputs(gate, value, lengths):
     _float_tensor(gate, 'gate', 3)
+    B, T, D = gate.shape
     if value is None:
-        if gate.shape[2] % 2:
+        if D % 2:
             raise ValueError('gate: without a value its channels are gate and value side by '
                              'side, an even number')
-        D = gate.shape[2] // 2
+        D //= 2
         gate, value = gate[..., :D], gate[..., D:]
     else:
         _float_tensor(value, 'value', 3, gate.dtype, gate.device)
         if value.shape != gate.shape:
             raise ValueError(f'value: {tuple(value.shape)}, gate: {tuple(gate.shape)}')
-    B, T, D = (int(n) for n in gate.shape)
     if D == 0:
         raise ValueError('gate: no channels')
     if lengths is not None:
@@ -1312,14 +1337,6 @@ def _lane_state(t, name, B, D, dev):
         if tuple(t.shape) != (B, D):
             raise ValueError(f'{name}: expected [{B},{D}], got {tuple(t.shape)}')
     return t
-
-
-def _workspace(bytes_, what, dev):
-    """Scratch memory of one call.  From torch's allocator every time: its blocks follow the
-    stream (and, under capture, belong to the graph), so no two calls share one."""
-    if bytes_ < 0:
-        _lib.check(int(bytes_), what)
-    return torch.empty((bytes_ + 3) // 4, dtype=torch.float32, device=dev) if bytes_ else None
 
 
 def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, state_out=None,
@@ -1341,22 +1358,20 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
             raise ValueError(f'out: expected {tuple(gate.shape)}, got {tuple(out.shape)}')
     last = _lane_state(state_out, 'state_out', B, D, dev)
     if last is None:
-        last = torch.empty(B, D, dtype=torch.float32, device=dev)
+        last = gate.new_empty((B, D), dtype=torch.float32)
     if B == 0 or T == 0:
         if last is not state:
             last.copy_(state) if state is not None else last.zero_()
         return out, last, None
     ckpt = None
     if want_ckpt and T > RECURRENCE_SPAN:
-        ckpt = torch.empty(-(-T // RECURRENCE_SPAN), B, D, dtype=torch.float32, device=dev)
+        ckpt = gate.new_empty((-(-T // RECURRENCE_SPAN), B, D), dtype=torch.float32)
     code = FLOAT_DTYPES[gate.dtype]
-    with torch.cuda.device(dev):
-        need = lib.tempo_recurrence_workspace(B, T, D, code, 0)
-        ws = _workspace(need, 'tempo_recurrence_workspace', dev)
-        rc = lib.tempo_recurrence(*_strided(gate), *_strided(value), _ptr(state), _ptr(lengths),
-                                  *_strided(out), _ptr(last), _ptr(ckpt), B, T, D, code,
-                                  _ptr(ws), need, _stream_ptr(dev))
-    _lib.check(rc, 'tempo_recurrence')
+    need = lib.tempo_recurrence_workspace(B, T, D, code, 0)
+    ws = _workspace(need, 'tempo_recurrence_workspace', gate)
+    _launch('tempo_recurrence', dev, lib.tempo_recurrence, *_strided(gate), *_strided(value),
+            _address(state), _address(lengths), *_strided(out), last.data_ptr(), _address(ckpt),
+            B, T, D, code, _address(ws), need)
     return out, last, ckpt
 
 
@@ -1365,44 +1380,52 @@ def recurrence_backward(grad_h, grad_last, gate, value=None, state=None, ckpt=No
     """Gradients of :func:`recurrence_forward`: ``(grad_gate, grad_value, grad_state)``;
     ``grad_value`` is None where gate and value came side by side (``grad_gate`` holds both).
     ``grad_h`` / ``grad_last`` None: zeros."""
-    lib = _lib.load()
-    both = value is None
-    packed = gate
-    gate, value, B, T, D = _recurrence_inputs(gate, value, lengths)
+    _, _, B, T, D = _recurrence_inputs(gate, value, lengths)
     dev = gate.device
-    if grad_h is None:
-        grad_h = torch.zeros(D, dtype=gate.dtype, device=dev).expand(B, T, D)
-    elif D > 1 and grad_h.stride(-1) != 1:
-        grad_h = grad_h.contiguous()
-    _float_tensor(grad_h, 'grad_h', 3, gate.dtype, dev)
-    if grad_h.shape != gate.shape:
-        raise ValueError(f'grad_h: expected {tuple(gate.shape)}, got {tuple(grad_h.shape)}')
+    if grad_h is not None:
+        if D > 1 and grad_h.stride(-1) != 1:
+            grad_h = grad_h.contiguous()
+        _float_tensor(grad_h, 'grad_h', 3, gate.dtype, dev)
+        if tuple(grad_h.shape) != (B, T, D):
+            raise ValueError(f'grad_h: expected {[B, T, D]}, got {list(grad_h.shape)}')
     _lane_state(grad_last, 'grad_last', B, D, dev)
     _lane_state(state, 'state', B, D, dev)
     if T > RECURRENCE_SPAN and B:
         _need(ckpt, torch.float32, 'ckpt', dev)
         if tuple(ckpt.shape) != (-(-T // RECURRENCE_SPAN), B, D):
             raise ValueError('ckpt has the wrong size')
+    return _recurrence_backward(grad_h, grad_last, gate, value, state, ckpt, lengths, want_state)
+
+
+def _recurrence_backward(grad_h, grad_last, gate, value, state, ckpt, lengths, want_state):
+    """The same on arguments that are known to fit (``grad_h``: channels adjacent)."""
+    both = value is None
+    B, T, D = gate.shape
+    dgate = _like_time_order(gate, D)
+    packed = dgate
+    if both:
+        D //= 2
+        gate, value = gate[..., :D], gate[..., D:]
+        dgate, dvalue = packed[..., :D], packed[..., D:]
     else:
-        ckpt = state
-    dpacked = _like_time_order(packed, int(packed.shape[2]))
-    dgate, dvalue = (dpacked[..., :D], dpacked[..., D:]) if both else \
-        (dpacked, _like_time_order(gate, D))
-    dstate = torch.empty(B, D, dtype=torch.float32, device=dev) if want_state else None
+        dvalue = _like_time_order(gate, D)
+    if grad_h is None:
+        grad_h = gate.new_zeros(D).expand(B, T, D)
+    dstate = gate.new_empty((B, D), dtype=torch.float32) if want_state else None
     if B == 0 or T == 0:
         if want_state:
             dstate.copy_(grad_last) if grad_last is not None else dstate.zero_()
     else:
+        lib = _lib.load()
         code = FLOAT_DTYPES[gate.dtype]
-        with torch.cuda.device(dev):
-            need = lib.tempo_recurrence_workspace(B, T, D, code, 1)
-            ws = _workspace(need, 'tempo_recurrence_workspace', dev)
-            rc = lib.tempo_recurrence_backward(
-                *_strided(gate), *_strided(value), *_strided(grad_h), _ptr(grad_last),
-                _ptr(lengths), _ptr(ckpt), *_strided(dgate), *_strided(dvalue), _ptr(dstate),
-                B, T, D, code, _ptr(ws), need, _stream_ptr(dev))
-        _lib.check(rc, 'tempo_recurrence_backward')
-    return dpacked, None if both else dvalue, dstate
+        need = lib.tempo_recurrence_workspace(B, T, D, code, 1)
+        ws = _workspace(need, 'tempo_recurrence_workspace', gate)
+        _launch('tempo_recurrence_backward', gate.device, lib.tempo_recurrence_backward,
+                *_strided(gate), *_strided(value), *_strided(grad_h), _address(grad_last),
+                _address(lengths), _address(ckpt if T > RECURRENCE_SPAN else state),
+                *_strided(dgate), *_strided(dvalue), _address(dstate), B, T, D, code,
+                _address(ws), need)
+    return packed, None if both else dvalue, dstate
 
 
 # --------------------------------------------------------------------------
@@ -1421,9 +1444,12 @@ def _activation(name):
 def _rows(t, name, dtype=None, device=None):
     """``[..., C]`` as ``[rows, C]`` without a copy: channels adjacent, one distance between
     rows."""
-    if isinstance(t, torch.Tensor) and t.dim() == 0:
+    dim = t.dim() if isinstance(t, torch.Tensor) else 0
+    if dim == 0 and isinstance(t, torch.Tensor):
         raise ValueError(f'{name}: no channels')
-    _float_tensor(t, name, t.dim() if isinstance(t, torch.Tensor) else 0, dtype, device)
+    _float_tensor(t, name, dim, dtype, device)
+    if dim == 2:
+        return t
     try:
         return t.view(t.numel() // max(t.shape[-1], 1), t.shape[-1])
     except RuntimeError:
@@ -1435,16 +1461,17 @@ def _linear_operands(x, weight, bias):
     rows = _rows(x, 'x')
     dtype, dev = x.dtype, x.device
     _float_tensor(weight, 'weight', 2, dtype, dev)
-    N, K = (int(n) for n in weight.shape)
-    if int(rows.shape[1]) != K:
-        raise ValueError(f'weight: expected [N,{int(rows.shape[1])}], got {tuple(weight.shape)}')
+    N, K = weight.shape
+    M = rows.shape[0]
+    if rows.shape[1] != K:
+        raise ValueError(f'weight: expected [N,{rows.shape[1]}], got {tuple(weight.shape)}')
     if N == 0 or K == 0:
         raise ValueError('weight: no channels')
     if bias is not None:
         _float_tensor(bias, 'bias', 1, dtype, dev)
-        if int(bias.shape[0]) != N:
+        if bias.shape[0] != N:
             raise ValueError(f'bias: expected [{N}], got {tuple(bias.shape)}')
-    return rows, int(rows.shape[0]), N, K
+    return rows, M, N, K
 
 
 def linear_forward(x, weight, bias=None, residual=None, activation='none', out=None,
@@ -1457,64 +1484,77 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
     act = _activation(activation)
     rows, M, N, K = _linear_operands(x, weight, bias)
     dev, code = x.device, FLOAT_DTYPES[x.dtype]
-    shape = tuple(x.shape[:-1]) + (N,)
-    res = None
+    shape = (*x.shape[:-1], N)
+    res, ldr = None, 0
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or tuple(residual.shape) != shape:
             raise ValueError(f'residual: expected {list(shape)}, got '
                              f'{list(getattr(residual, "shape", []))}')
         res = _rows(residual, 'residual', x.dtype, dev)
+        ldr = res.stride(0)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-    elif tuple(out.shape) != shape:
-        raise ValueError(f'out: expected {list(shape)}, got {list(out.shape)}')
-    dst = _rows(out, 'out', x.dtype, dev)
-    if M > 1 and dst.stride(0) < N:
-        raise ValueError('out: its rows overlap')
-    pre = torch.empty(M, N, dtype=x.dtype, device=dev) if want_pre and act else None
+        out = dst = x.new_empty(shape)
+        ldy = N
+    else:
+        if tuple(out.shape) != shape:
+            raise ValueError(f'out: expected {list(shape)}, got {list(out.shape)}')
+        dst = _rows(out, 'out', x.dtype, dev)
+        ldy = dst.stride(0)
+        if M > 1 and ldy < N:
+            raise ValueError('out: its rows overlap')
+    pre = x.new_empty((M, N)) if want_pre and act else None
     if M == 0:
         return out, pre
-    with torch.cuda.device(dev):
-        need = lib.tempo_linear_workspace(M, N, K, code, act, 0)
-        ws = _workspace(need, 'tempo_linear_workspace', dev)
-        rc = lib.tempo_linear(_ptr(rows), rows.stride(0), _ptr(weight), weight.stride(0),
-                              _ptr(bias), _ptr(res), 0 if res is None else res.stride(0),
-                              _ptr(dst), dst.stride(0), _ptr(pre), M, N, K, code, act, _ptr(ws),
-                              need, _stream_ptr(dev))
-    _lib.check(rc, 'tempo_linear')
+    need = lib.tempo_linear_workspace(M, N, K, code, act, 0)
+    ws = _workspace(need, 'tempo_linear_workspace', x)
+    _launch('tempo_linear', dev, lib.tempo_linear, rows.data_ptr(), rows.stride(0),
+            weight.data_ptr(), weight.stride(0), _address(bias), _address(res), ldr,
+            dst.data_ptr(), ldy, _address(pre), M, N, K, code, act, _address(ws), need)
     return out, pre
 
 
 def linear_backward(grad_y, x, weight, pre=None, activation='none', want=(True, True, True)):
     """Gradients of :func:`linear_forward` with respect to x, weight and bias, each None where
     ``want`` says so; the residual's is ``grad_y`` itself."""
-    lib = _lib.load()
     act = _activation(activation)
-    rows, M, N, K = _linear_operands(x, weight, None)
-    dev, code = x.device, FLOAT_DTYPES[x.dtype]
-    if tuple(grad_y.shape) != tuple(x.shape[:-1]) + (N,):
-        raise ValueError(f'grad_y: expected {list(x.shape[:-1]) + [N]}, got '
-                         f'{list(grad_y.shape)}')
-    try:
-        g = _rows(grad_y, 'grad_y', x.dtype, dev)
-    except ValueError:  # e.g. the gradient of a sum: no memory of its own
-        g = _rows(grad_y.contiguous(), 'grad_y', x.dtype, dev)
+    _, M, N, _ = _linear_operands(x, weight, None)
+    if tuple(grad_y.shape) != (*x.shape[:-1], N):
+        raise ValueError(f'grad_y: expected {[*x.shape[:-1], N]}, got {list(grad_y.shape)}')
+    _float_tensor(grad_y.reshape(-1)[:0], 'grad_y', 1, x.dtype, x.device)
     if act and M:
-        _need(pre, x.dtype, 'pre', dev)
+        _need(pre, x.dtype, 'pre', x.device)
         if tuple(pre.shape) != (M, N):
             raise ValueError(f'pre: expected [{M},{N}], got {tuple(pre.shape)}')
-    make = torch.empty if M else torch.zeros
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want[0] else None
-    dw = make(N, K, dtype=x.dtype, device=dev) if want[1] else None
-    db = make(N, dtype=x.dtype, device=dev) if want[2] else None
-    if M == 0 or not any(want):
+    return _linear_backward(grad_y, x, weight, pre, act, want)
+
+
+def _linear_backward(grad_y, x, weight, pre, act, want):
+    """The same on arguments that are known to fit (``grad_y``: any strides)."""
+    N, K = weight.shape
+    M = x.numel() // K
+    dx = x.new_empty(x.shape) if want[0] else None
+    dw = weight.new_empty((N, K)) if want[1] else None
+    db = weight.new_empty(N) if want[2] else None
+    if M == 0:
+        for t in (dw, db):
+            if t is not None:
+                t.zero_()
+    if M == 0 or (dx is None and dw is None and db is None):
         return dx, dw, db
-    with torch.cuda.device(dev):
-        need = lib.tempo_linear_workspace(M, N, K, code, act, 1)
-        ws = _workspace(need, 'tempo_linear_workspace', dev)
-        rc = lib.tempo_linear_backward(_ptr(g), g.stride(0), _ptr(pre), _ptr(rows),
-                                       rows.stride(0), _ptr(weight), weight.stride(0), _ptr(dx),
-                                       K, _ptr(dw), _ptr(db), M, N, K, code, act, _ptr(ws),
-                                       need, _stream_ptr(dev))
-    _lib.check(rc, 'tempo_linear_backward')
+    ldx = x.stride(0) if x.dim() == 2 else x.view(M, K).stride(0)
+    if grad_y.is_contiguous():
+        ldg = N
+    else:
+        try:
+            grad_y = _rows(grad_y, 'grad_y')
+        except ValueError:  # e.g. the gradient of a sum: no memory of its own
+            grad_y = grad_y.contiguous().view(M, N)
+        ldg = grad_y.stride(0)
+    lib = _lib.load()
+    code = FLOAT_DTYPES[x.dtype]
+    need = lib.tempo_linear_workspace(M, N, K, code, act, 1)
+    ws = _workspace(need, 'tempo_linear_workspace', x)
+    _launch('tempo_linear_backward', x.device, lib.tempo_linear_backward, grad_y.data_ptr(), ldg,
+            _address(pre), x.data_ptr(), ldx, weight.data_ptr(), weight.stride(0), _address(dx),
+            K, _address(dw), _address(db), M, N, K, code, act, _address(ws), need)
     return dx, dw, db

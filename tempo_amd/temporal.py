@@ -34,10 +34,12 @@ class _GatedRecurrence(torch.autograd.Function):
             return None, None, None, None
         gate, value, state, ckpt, lengths = ctx.saved_tensors
         need = ctx.needs_input_grad
+        if grad_h is not None and grad_h.stride(2) != 1:
+            grad_h = grad_h.contiguous()
         if grad_last is not None:
             grad_last = grad_last.contiguous()
-        dgate, dvalue, dstate = ops.recurrence_backward(grad_h, grad_last, gate, value, state,
-                                                        ckpt, lengths, want_state=need[2])
+        dgate, dvalue, dstate = ops._recurrence_backward(grad_h, grad_last, gate, value, state,
+                                                         ckpt, lengths, need[2])
         return (dgate if need[0] else None, dvalue if need[1] else None,
                 dstate if need[2] else None, None)
 
@@ -78,7 +80,7 @@ class _FusedLinear(torch.autograd.Function):
     def forward(ctx, x, weight, bias, residual, activation):
         y, pre = ops.linear_forward(x, weight, bias, residual, activation, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
-        ctx.activation = activation
+        ctx.activation = ops.ACTIVATIONS[activation]
         return y
 
     @staticmethod
@@ -86,7 +88,7 @@ class _FusedLinear(torch.autograd.Function):
     def backward(ctx, grad_y):
         x, weight, pre = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dx, dw, db = ops.linear_backward(grad_y, x, weight, pre, ctx.activation, need[:3])
+        dx, dw, db = ops._linear_backward(grad_y, x, weight, pre, ctx.activation, need)
         return dx, dw, db, grad_y if need[3] else None, None
 
 
