@@ -897,10 +897,11 @@ struct ThinArgs {
 };
 
 template <typename T, int NJ>
-__global__ __launch_bounds__(kThreads) void thin_kernel(const ThinArgs<T> args) {
+__global__ __launch_bounds__(kThreads, 3) void thin_kernel(const ThinArgs<T> args) {
   constexpr int E = 16 / sizeof(T), kStep = 2 * E;
-  constexpr int kPair = NJ < 2 ? 1 : 2;  // column blocks that pass through LDS together
-  constexpr uint32_t kQuads = kPair * 8;
+  constexpr uint32_t kQuads = 8;
+  // rows of the epilogue under way at a time: what 168 registers hold without spills
+  constexpr int kThinTogether = NJ == 2 && sizeof(T) == 4 ? 1 : 2;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TileArgs& a = args.t;
   const uint32_t lane = threadIdx.x % 64;
@@ -923,7 +924,7 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(const ThinArgs<T> args) 
     *reinterpret_cast<u32x4*>(lds + (size_t)q * 16) = v;
   }
   __syncthreads();
-  char* turn = lds + (size_t)NJ * args.steps * 1024 + wave * (kPair * 4096);
+  char* turn = lds + (size_t)NJ * args.steps * 1024 + wave * 4096;
 
   const uint32_t chunks = (args.steps + kChunk - 1) / kChunk;
   const uint32_t stride = gridDim.x * (kThreads / 64);
@@ -968,39 +969,36 @@ __global__ __launch_bounds__(kThreads) void thin_kernel(const ThinArgs<T> args) 
     const long long left = a.I - (long long)blk * 32;
     const uint32_t high = (uint32_t)min(32ll, left);
 #pragma unroll
-    for (int y0 = 0; y0 < NJ; y0 += kPair) {
+    for (int y = 0; y < NJ; ++y) {
 #pragma unroll
-      for (int y = 0; y < kPair; ++y) {
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t i = lane % 32, q = 2 * g + lane / 32;
+        f32x4 v;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t i = lane % 32, q = y * 8 + 2 * g + lane / 32;
-          f32x4 v;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            v[r] = acc[y0 + y][4 * g + r];
-            acc[y0 + y][4 * g + r] = 0.f;
-          }
-          *reinterpret_cast<f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16) = v;
+        for (int r = 0; r < 4; ++r) {
+          v[r] = acc[y][4 * g + r];
+          acc[y][4 * g + r] = 0.f;
         }
+        *reinterpret_cast<f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16) = v;
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       const uint32_t q = lane % kQuads;
-      const long long j = y0 * 32 + q * 4;
+      const long long j = y * 32 + q * 4;
       const int n = (int)min(4ll, a.J - j);
       if (n > 0) {
         constexpr uint32_t kApart = 64 / kQuads;
 #pragma unroll 1
-        for (uint32_t i = lane / kQuads; i < high; i += kTogether * kApart) {
-          f32x4 v[kTogether];
+        for (uint32_t i = lane / kQuads; i < high; i += kThinTogether * kApart) {
+          f32x4 v[kThinTogether];
 #pragma unroll
-          for (int r = 0; r < kTogether; ++r) {
+          for (int r = 0; r < kThinTogether; ++r) {
             const uint32_t row = i + r * kApart;  // < 32, the block's rows
             v[r] = *reinterpret_cast<const f32x4*>(
                 turn + (row * kQuads + (q ^ (row % kQuads))) * 16);
           }
-          finish<T, kTogether>(a.e, (long long)blk * 32 + i, kApart, a.I, j, n, v);
+          finish<T, kThinTogether>(a.e, (long long)blk * 32 + i, kApart, a.I, j, n, v);
         }
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -1116,53 +1114,91 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const TileArgs a) {
 
 constexpr int kRowsPerBlock = 512;
 
+template <bool FULL, int V, typename Chunk>
+__device__ __forceinline__ void slopes(const Chunk& z, float (&d)[V], int act) {
+  switch (act) {  // one branch for all of them
+#define TEMPO_EACH(name)                                                            \
+  case name:                                                                        \
+    _Pragma("unroll") for (int q = 0; q < V; ++q) d[q] = slope<FULL>((float)z[q], name); \
+    break;
+    TEMPO_EACH(RELU)
+    TEMPO_EACH(SILU)
+    TEMPO_EACH(GELU)
+    TEMPO_EACH(SIGMOID)
+    TEMPO_EACH(TANH)
+#undef TEMPO_EACH
+    default: break;
+  }
+}
+
 // dz = g * act'(z) in the tensors' type (unless dz is NULL) and the sums of the unrounded
-// values over the workgroup's rows.  A thread owns 4 columns, 8 threads side by side.
+// values over the workgroup's rows.  A thread owns 16 bytes of columns, 8 threads side by side,
+// four rows of each under way at a time.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long ldg, const T* pre,
                                                           T* dz, float* sums, long long M, int N,
                                                           int act) {
   constexpr bool FULL = sizeof(T) == 4;
-  __shared__ float s_sum[32][33];
-  const int j = blockIdx.y * 32 + threadIdx.x % 8 * 4;
+  constexpr int V = 16 / sizeof(T), kWide = 8 * V, kRows = 4;
+  typedef typename Pack<T, V>::type Chunk;
+  __shared__ float s_sum[kWide][33];
+  const int j = blockIdx.y * kWide + threadIdx.x % 8 * V;
   const int r = threadIdx.x / 8;
   const long long first = (long long)blockIdx.x * kRowsPerBlock;
   const long long stop = min(M, first + kRowsPerBlock);
-  const int n = max(0, min(4, N - j));
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (long long i = first + r; i < stop; i += 32) {
-    if (n == 4) {
-      typedef typename Pack<T, 4>::type V4;
-      const V4 gv = *reinterpret_cast<const V4*>(g + i * ldg + j);
-      V4 zv = gv, out;
-      if (pre) zv = *reinterpret_cast<const V4*>(pre + i * N + j);
+  const int n = max(0, min(V, N - j));
+  float sum[V];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float d = (float)gv[q] * slope<FULL>((float)zv[q], act);
-        sum[q] += d;
-        out[q] = (T)d;
+  for (int q = 0; q < V; ++q) sum[q] = 0.f;
+  if (n > 0) {
+    for (long long i0 = first + r; i0 < stop; i0 += 32 * kRows) {
+      Chunk gv[kRows], zv[kRows];
+#pragma unroll
+      for (int x = 0; x < kRows; ++x) {
+        const long long i = min(i0 + 32 * x, stop - 1);
+        if (n == V) {
+          gv[x] = *reinterpret_cast<const Chunk*>(g + i * ldg + j);
+          if (pre) zv[x] = *reinterpret_cast<const Chunk*>(pre + i * N + j);
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q) {
+            gv[x][q] = q < n ? g[i * ldg + j + q] : (T)0.f;
+            if (pre) zv[x][q] = q < n ? pre[i * N + j + q] : (T)0.f;
+          }
+        }
       }
-      if (dz) *reinterpret_cast<V4*>(dz + i * N + j) = out;
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (q < n) {
-          const float z = pre ? (float)pre[i * N + j + q] : 0.f;
-          const float d = (float)g[i * ldg + j + q] * slope<FULL>(z, act);
-          sum[q] += d;
-          if (dz) dz[i * N + j + q] = (T)d;
+      for (int x = 0; x < kRows; ++x) {
+        const long long i = i0 + 32 * x;
+        if (i >= stop) continue;
+        float d[V];
+        if (pre) slopes<FULL, V>(zv[x], d, act);
+        Chunk out;
+#pragma unroll
+        for (int q = 0; q < V; ++q) {
+          d[q] = (float)gv[x][q] * (pre ? d[q] : 1.f);
+          sum[q] += d[q];
+          out[q] = (T)d[q];
+        }
+        if (!dz) continue;
+        if (n == V) {
+          *reinterpret_cast<Chunk*>(dz + i * N + j) = out;
+        } else {
+#pragma unroll
+          for (int q = 0; q < V; ++q)
+            if (q < n) dz[i * N + j + q] = out[q];
         }
       }
     }
   }
   if (!sums) return;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) s_sum[threadIdx.x % 8 * 4 + q][r] = sum[q];
+  for (int q = 0; q < V; ++q) s_sum[threadIdx.x % 8 * V + q][r] = sum[q];
   __syncthreads();
-  if (threadIdx.x < 32) {
+  if (threadIdx.x < kWide) {
     float total = 0.f;
     for (int k = 0; k < 32; ++k) total += s_sum[threadIdx.x][k];
-    const int col = blockIdx.y * 32 + threadIdx.x;
+    const int col = blockIdx.y * kWide + threadIdx.x;
     if (col < N) sums[(long long)blockIdx.x * N + col] = total;
   }
 }
@@ -1205,18 +1241,16 @@ struct Product {
 };
 
 constexpr int kFewRows = 64;
-constexpr int kThinColumns = 256;
+constexpr int kThinColumns = 64;
 constexpr long long kThinRows = 16384;
 constexpr uint32_t kThinLds = 81920;  // half a compute unit's: two workgroups share one
 
-uint32_t thin_blocks(long long J) {  // 32-column blocks: 1, 2, 4 or 8
-  return J <= 32 ? 1 : J <= 64 ? 2 : J <= 128 ? 4 : 8;
-}
+uint32_t thin_blocks(long long J) { return J <= 32 ? 1 : 2; }  // of 32 columns
 
 uint32_t thin_lds(long long J, long long K, int size) {
   const uint32_t nj = thin_blocks(J);
   const long long steps = (K * size + 31) / 32;
-  const long long bytes = nj * steps * 1024 + 4 * (nj < 2 ? 1 : 2) * 4096;
+  const long long bytes = nj * steps * 1024 + 4 * 4096;
   return bytes > kThinLds ? 0 : (uint32_t)bytes;
 }
 
@@ -1297,7 +1331,7 @@ int run_few(const TileArgs& t, hipStream_t stream) {
 template <typename T, int NJ>
 void launch_thin(const ThinArgs<T>& a, uint32_t lds, hipStream_t stream) {
   const uint32_t groups = (a.blocks + 3) / 4;
-  const dim3 grid(groups < 2 * kUnits ? groups : 2 * kUnits);
+  const dim3 grid(groups < 3 * kUnits ? groups : 3 * kUnits);
   hipLaunchKernelGGL((thin_kernel<T, NJ>), grid, dim3(kThreads), lds, stream, a);
 }
 
@@ -1309,12 +1343,8 @@ int run_thin(const TileArgs& t, int b_layout, hipStream_t stream) {
   a.steps = (uint32_t)((t.K * (long long)sizeof(T) + 31) / 32);
   a.b_layout = b_layout;
   const uint32_t lds = thin_lds(t.J, t.K, sizeof(T));
-  switch (thin_blocks(t.J)) {
-    case 1: launch_thin<T, 1>(a, lds, stream); break;
-    case 2: launch_thin<T, 2>(a, lds, stream); break;
-    case 4: launch_thin<T, 4>(a, lds, stream); break;
-    default: launch_thin<T, 8>(a, lds, stream); break;
-  }
+  if (thin_blocks(t.J) == 1) launch_thin<T, 1>(a, lds, stream);
+  else launch_thin<T, 2>(a, lds, stream);
   return (int)hipGetLastError();
 }
 
@@ -1408,8 +1438,8 @@ int backward_for(const BackwardPlan& p, const void* g, long long ldg, const void
   float* scratch = (float*)(ws + p.dz_bytes + p.sum_bytes);
   const long long blocks = (M + kRowsPerBlock - 1) / kRowsPerBlock;
   if (dz || db) {
-    hipLaunchKernelGGL((grad_z_kernel<T>), dim3((unsigned)blocks, (N + 31) / 32), dim3(kThreads),
-                       0, stream, (const T*)g, ldg, (const T*)pre, dz, sums, M, N, act);
+    hipLaunchKernelGGL((grad_z_kernel<T>), dim3((unsigned)blocks, (N + 128 / (int)sizeof(T) - 1) / (128 / (int)sizeof(T))),
+                       dim3(kThreads), 0, stream, (const T*)g, ldg, (const T*)pre, dz, sums, M, N, act);
     if (db)
       hipLaunchKernelGGL((grad_bias_kernel<T>), dim3((N + 7) / 8), dim3(kThreads), 0, stream,
                          sums, blocks, N, (T*)db);
