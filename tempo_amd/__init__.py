@@ -5,8 +5,8 @@ modules, running hand-written HIP kernels (gfx950) through a C ABI, and the
 temporal head's operators that go in front of them.
 """
 from .project_layer import (PackedHeatmaps, ProcessLayerNHWC, ProjectLayer,  # noqa: F401
-                            ProjectLayerWithMask)
+                            ProjectLayerWithMask, RecurrentProcessLayerNHWC)
 from .temporal import fused_linear, gated_recurrence  # noqa: F401
 
 __all__ = ['ProjectLayer', 'ProjectLayerWithMask', 'ProcessLayerNHWC', 'PackedHeatmaps',
-           'fused_linear', 'gated_recurrence']
+           'RecurrentProcessLayerNHWC', 'fused_linear', 'gated_recurrence']

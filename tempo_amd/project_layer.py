@@ -25,6 +25,7 @@ import torch.nn as nn
 
 from . import ops
 from .camera import pack_cameras, to_device
+from .temporal import fused_linear, gated_recurrence
 
 
 def _pair(v):
@@ -83,6 +84,41 @@ class ProcessLayerNHWC(nn.Module):
         B = hm.shape[0] // timesteps
         C = int(self.weight.shape[0])
         return [PackedHeatmaps(hm[t * B:(t + 1) * B], C) for t in range(timesteps)]
+
+
+class RecurrentProcessLayerNHWC(nn.Module):
+    """:class:`ProcessLayerNHWC` with a memory over timesteps: the 1x1 convolution yields a gate
+    and a candidate per channel, and every texel's features follow the GRU's update
+    ``h_t = (1 - z_t) h_{t-1} + z_t v_t`` (the reference's temporal cell,
+    ``fiery_temporal.py:109``) with gates from the current maps alone.
+
+    ``weight [2C,K,1,1]`` and ``bias [2C]``: the gates' C output channels first, then the
+    candidates'.  ``forward(backbone_map, num_views, timesteps, state)`` takes the maps of all
+    ``T*V*B`` images as ``rnn_multiview_pose.py:321`` stacks them (a ``torch.channels_last`` map
+    is read where it lies, another one is copied into that order) and returns
+    ``(feature_maps, state)``: ``feature_maps[t][v]`` is ``[B,C,H,W]`` in channels_last memory,
+    which the project layers read in place, and ``state`` (fp32 ``[V*B*H*W, C]``) goes into the
+    next call, so that a recording can be fed one timestep at a time.  Trains through both
+    operators (:mod:`tempo_amd.temporal`); half-precision maps run in their own type."""
+
+    def __init__(self, in_channels=256, out_channels=32):
+        super().__init__()
+        conv = nn.Conv2d(in_channels, 2 * out_channels, kernel_size=1)
+        self.weight, self.bias = conv.weight, conv.bias
+
+    def forward(self, backbone_map, num_views, timesteps=1, state=None):
+        images, K, H, W = backbone_map.shape
+        T, V = int(timesteps), int(num_views)
+        if images % (T * V):
+            raise ValueError('backbone_map.shape[0] must be timesteps * num_views * batch')
+        B, C = images // (T * V), int(self.weight.shape[0]) // 2
+        rows = backbone_map.contiguous(memory_format=torch.channels_last).permute(0, 2, 3, 1)
+        both = fused_linear(rows.reshape(-1, K), self.weight.to(backbone_map.dtype),
+                            self.bias.to(backbone_map.dtype))
+        # one lane per view, batch item, texel and channel; time outermost in memory
+        h, state = gated_recurrence(both.view(T, -1, 2 * C).transpose(0, 1), state=state)
+        maps = h.transpose(0, 1).view(T, V, B, H, W, C).permute(0, 1, 2, 5, 3, 4)
+        return [[maps[t, v] for v in range(V)] for t in range(T)], state
 
 
 def _packed_sequence(feature_maps_t):

@@ -1,0 +1,155 @@
+"""The temporal head as it is used: backbone maps through the recurrent process layer into the
+unprojection, trained and streamed."""
+import pytest
+import torch
+
+import cases
+import temporal_ref as R
+
+pytestmark = pytest.mark.gpu
+
+K, C, T = 24, 15, 3
+
+
+def _head(dev, dtype=torch.float32, seed=0, hw=(14, 24), V=5, B=2):
+    import tempo_amd
+    gen = torch.Generator().manual_seed(seed)
+    head = tempo_amd.RecurrentProcessLayerNHWC(K, C)
+    with torch.no_grad():
+        head.weight.copy_(torch.randn(head.weight.shape, generator=gen) / K ** 0.5)
+        head.bias.copy_(torch.randn(head.bias.shape, generator=gen) * 0.3)
+    maps = torch.randn(T * V * B, K, *hw, generator=gen).to(dtype)
+    return head.to(dev), maps.to(dev)
+
+
+def _reference(head, maps, V, state=None, grads=None):
+    """Both operators in 64 bits; tolerances of the run of the two: the product's error enters
+    the recurrence as one of its inputs, which it scales by at most 1 (value) and by
+    |v - h| / 4 (gate) at each step, over all steps that are not forgotten."""
+    images, _, H, W = maps.shape
+    rows = maps.permute(0, 2, 3, 1).reshape(-1, K)
+    w, b = (p.detach().to(maps.dtype) for p in (head.weight.flatten(1), head.bias))
+    lin = R.linear(rows, w, b)
+    both = lin['y'].view(T, -1, 2 * C).transpose(0, 1)
+    tol = lin['y_tol'].view(T, -1, 2 * C).transpose(0, 1)
+    rec = R.recurrence(both[..., :C].to(maps.dtype), both[..., C:].to(maps.dtype), state)
+    peak = both[..., C:].abs().amax(dim=1, keepdim=True)
+    if state is not None:
+        peak = torch.maximum(peak, state.double().cpu().abs()[:, None])
+    # the reference itself rounds the product once, the kernel once: twice the tolerance
+    moved = 2 * T * (tol[..., C:].amax(1, keepdim=True) +
+                     tol[..., :C].amax(1, keepdim=True) * 2 * peak / 4)
+    return lin, rec, both, moved
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('memory', [torch.contiguous_format, torch.channels_last], ids=str)
+def test_recurrent_process_layer_maps(memory, dtype, gpu_device):
+    V, B = 5, 2
+    head, maps = _head(gpu_device, dtype)
+    with torch.no_grad():
+        out, state = head(maps.contiguous(memory_format=memory), V, T)
+    assert len(out) == T and all(len(m) == V for m in out)
+    _, rec, _, moved = _reference(head, maps, V)
+    H, W = maps.shape[2:]
+    got = torch.stack([torch.stack(m) for m in out])  # [T,V,B,C,H,W]
+    got = got.permute(1, 2, 4, 5, 0, 3).reshape(-1, T, C)
+    R.check(got, rec['h'], rec['h_tol'] + moved, 'maps')
+    R.check(state, rec['last'], rec['last_tol'] + moved[:, 0], 'state')
+    assert out[0][0].shape == (B, C, H, W)
+    assert out[0][0].is_contiguous(memory_format=torch.channels_last)
+
+
+def test_one_timestep_at_a_time(gpu_device):
+    V = 5
+    head, maps = _head(gpu_device)
+    per = maps.shape[0] // T
+    with torch.no_grad():
+        whole, last = head(maps, V, T)
+        state = None
+        for t in range(T):
+            step, state = head(maps[t * per:(t + 1) * per], V, 1, state)
+            _, rec, _, moved = _reference(head, maps, V)
+            tol = (rec['h_tol'] + moved)[:, t]
+            for v in range(V):
+                a, b = step[0][v].double().cpu(), whole[t][v].double().cpu()
+                lim = tol.view(V, -1, *maps.shape[2:], C)[v].permute(0, 3, 1, 2)
+                assert bool(((a - b).abs() <= 2 * lim).all())
+    assert state.shape == last.shape
+
+
+def test_head_and_unprojection_together(gpu_device):
+    """Maps go into the root volume where they lie, with the values of NCHW copies; the
+    gradients of a loss on the volume reach the head's parameters and the backbone's maps."""
+    import tempo_amd
+    spec = dict(cfg='panoptic', B=2, cube=[12, 10, 9], hm='noise', joints=C, seed=900)
+    case = cases.to_device(cases.build_root(None, full=spec), gpu_device)
+    V = len(case['args'][0])
+    hw = tuple(case['args'][0][0].shape[2:])
+    head, maps = _head(gpu_device, hw=hw, V=V)
+    layer = tempo_amd.ProjectLayer(case['image_size'], case['heatmap_size'], 'mean')
+    rest = case['args'][1:]
+    maps.requires_grad_(True)
+    out, _ = head(maps, V, T)
+
+    def volume(m):
+        return torch.stack([layer(m[t], *rest)[0] for t in range(T)])
+
+    with torch.no_grad():
+        in_place = volume(out)
+        copied = volume([[m.contiguous() for m in ms] for ms in out])
+    assert torch.equal(in_place, copied)
+
+    gen = torch.Generator(device=gpu_device).manual_seed(1)
+    seed = torch.randn(in_place.shape, generator=gen, device=gpu_device)
+    leaves = [[m.detach().requires_grad_(True) for m in ms] for ms in out]
+    flat = [m for ms in leaves for m in ms]
+    g_maps = torch.autograd.grad(volume(leaves), flat, seed)
+    params = [head.weight, head.bias, maps]
+    mine = torch.autograd.grad([m for ms in out for m in ms], params, g_maps, retain_graph=True)
+
+    lin, rec, both, moved = _reference(head, maps.detach(), V)
+    g = torch.stack(list(g_maps)).view(T, V, -1, C, *hw).permute(1, 2, 4, 5, 0, 3)
+    g = g.reshape(-1, T, C)
+    back = R.recurrence(both[..., :C].float(), both[..., C:].float(), None, None, g, None)
+    d_both = torch.cat([back['dgate'], back['dvalue']], -1)
+    # the kernel's gates and values are off by `moved`: sigmoid and its slope change by at most
+    # a quarter of that, the states by `moved` itself
+    e = torch.cat([back['dgate_tol'], back['dvalue_tol']], -1)
+    peak = both.abs().amax(dim=1, keepdim=True)[..., C:]
+    size = g.double().cpu().abs().flip(1).cumsum(1).flip(1)
+    e = e + torch.cat([moved * size * (1 + 2 * peak), moved * size], -1) * T
+    rows = maps.detach().permute(0, 2, 3, 1).reshape(-1, K)
+    d_rows = d_both.transpose(0, 1).reshape(-1, 2 * C)
+    e_rows = e.transpose(0, 1).reshape(-1, 2 * C)
+    ref = R.linear(rows, head.weight.detach().flatten(1), head.bias.detach(), None, 'none',
+                   d_rows.float())
+    W64 = head.weight.detach().flatten(1).double().cpu()
+    X64 = rows.double().cpu()
+    R.check(mine[0].flatten(1), ref['dweight'], ref['dweight_tol'] + e_rows.t() @ X64.abs(),
+            'weight')
+    R.check(mine[1], ref['dbias'], ref['dbias_tol'] + e_rows.sum(0), 'bias')
+    R.check(mine[2].permute(0, 2, 3, 1).reshape(-1, K), ref['dx'],
+            ref['dx_tol'] + e_rows @ W64.abs(), 'backbone maps')
+
+    # the same in one go.  The unprojection's atomics add a texel's at most 12 x 10 x 9 terms in
+    # another order: each sum moves by at most 1080 x 2^-24 of its terms' magnitudes, and what
+    # follows is linear in it
+    whole = torch.autograd.grad(volume(out), params, seed)
+    size = torch.autograd.grad(volume(leaves), flat, seed.abs())
+    grown = torch.autograd.grad([m for ms in head(maps, V, T)[0] for m in ms], params,
+                                [1080 * 2.0 ** -24 * m.abs() for m in size])
+    for a, b, lim in zip(whole, mine, grown):
+        assert float((a - b).norm()) <= 4 * float(lim.norm()) + 1e-6 * float(b.norm())
+
+
+def test_parameters_and_refusals(gpu_device):
+    head, maps = _head(gpu_device)
+    assert sorted(head.state_dict()) == ['bias', 'weight']
+    assert tuple(head.weight.shape) == (2 * C, K, 1, 1)
+    with pytest.raises(ValueError):
+        head(maps, 7, T)
+    with pytest.raises(ValueError):
+        head(maps, 5, T, state=torch.zeros(3, C, device=gpu_device))
+    with pytest.raises(TypeError):
+        head(maps.cpu(), 5, T)
