@@ -318,7 +318,7 @@ __device__ __forceinline__ void activate_rows(f32x4 (&z)[ROWS], int act) {
 // The epilogue of ROWS quads of one column group, rows `apart` from each other, those from
 // `stop` on left out; n of the 4 columns are inside the matrix.  The residuals of all of them
 // are on their way before the first one is needed: one at a time, their latency took longer
-// than the products (256 x 256 tiles of 16384 x 4096 x 4096: 590 us against 415).
+// than four rows' (16384 x 4096 x 4096 with residual: 590 us against 544).
 template <typename T, int ROWS>
 __device__ __forceinline__ void finish(const Epilogue& e, long long i, uint32_t apart,
                                        long long stop, long long j, int n, f32x4 (&z)[ROWS]) {
@@ -1025,7 +1025,8 @@ __global__ __launch_bounds__(kThreads, 3) void thin_kernel(const ThinArgs<T> arg
 
 // ------------------------------------------------------------------------ few rows, any weight
 //
-// I <= 16 NI: what counts is reading B, once and by the whole card.  A workgroup takes 16 rows
+// I <= 16 NI: what counts is reading B, once and by the whole card (8 x 4096 x 4096 in fp16:
+// 11 us = 3.0 TB/s).  A workgroup takes 16 rows
 // of B; its waves share out k, each streaming its part of the 16 rows into the matrix units'
 // operands, and their sums meet in LDS.  One launch, no scratch memory.
 template <typename T>
@@ -1225,10 +1226,19 @@ __global__ __launch_bounds__(kThreads) void grad_bias_kernel(const float* sums, 
 
 constexpr int kUnits = 256;  // compute units to fill
 
-// Which kernel runs a product, by sizes and alignment alone:
-//   FEW    few rows, both operands with k adjacent (forward)
-//   THIN   many rows, few columns, A with k adjacent (forward, dx)
-//   TILE   anything;  STREAM_*  both operands aligned, by the tile's rows x columns
+// Which kernel runs a product, by sizes and alignment alone.  Measured with the rule and with
+// the other side of it, in us:
+//   FEW    up to kFewRows rows, both operands with k adjacent (forward).  8 x 4096 x 4096 in bf16
+//          10 against 15 (split tiles), 64 rows 22 against 24; in fp32 53 against 50
+//   THIN   from kThinRows rows on, up to kThinColumns columns, A with k adjacent, B within half
+//          of the LDS.  65536 x 32 x 256 in fp32 22 against 42, 4096 rows 17 against 22;
+//          wider outputs lose (dx of 614400 x 32 x 256 in bf16, 256 columns: 115 against 167)
+//   STREAM_32x256  both operands aligned, A's rows adjacent, at most 32 of them (the weight's
+//          gradient of a thin layer).  153600 x 32 x 256 in fp32 44 against 91, in bf16 75
+//          against 71 of which memory takes 74
+//   STREAM_256     both aligned, 16 bits, a 256 x 256 tile for every compute unit.  4096 x 4096 x
+//          1024 (256 tiles) 40 against 50 with 128 x 128; 4096 x 2048 x 2048 (128) 64 against 46
+//   STREAM_128     both aligned;   TILE  anything
 enum Kernel { FEW, THIN, TILE, STREAM_32x256, STREAM_128, STREAM_256 };
 
 struct Product {
@@ -1242,7 +1252,7 @@ struct Product {
 
 constexpr int kFewRows = 64;
 constexpr int kThinColumns = 64;
-constexpr long long kThinRows = 16384;
+constexpr long long kThinRows = 2048;
 constexpr uint32_t kThinLds = 81920;  // half a compute unit's: two workgroups share one
 
 uint32_t thin_blocks(long long J) { return J <= 32 ? 1 : 2; }  // of 32 columns
@@ -1293,7 +1303,8 @@ bool plan_product(long long I, long long J, long long K, int al, int bl, int dty
   p->tj = (uint32_t)tj;
   const long long depth = 128 / size;
   const long long steps = (K + depth - 1) / depth;
-  long long split = 2 * kUnits / (ti * tj);
+  const long long fill = p->kernel == STREAM_256 ? kUnits : 2 * kUnits;  // workgroups at a time
+  long long split = fill / (ti * tj);
   if (split > steps / 4) split = steps / 4;
   if (split < 1) split = 1;
   const long long part = (steps + split - 1) / split;
