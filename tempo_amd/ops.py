@@ -1301,6 +1301,19 @@ def _strided(t):
     return t.data_ptr(), t.stride(0), t.stride(1)
 
 
+def _apart(name, out, **inputs):
+    """Results are written while inputs are still read: they must not share memory."""
+    def ends(t):
+        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    if not out.numel():
+        return
+    low, high = ends(out)
+    for other, t in inputs.items():
+        if t is not None and t.numel() and ends(t)[0] < high and low < ends(t)[1]:
+            raise ValueError(f'{name}: shares memory with {other}')
+
+
 def _like_time_order(t, channels):
     """Empty ``[B,T,channels]`` whose memory has time outermost where ``t``'s has."""
     B, T, _ = t.shape
@@ -1356,8 +1369,12 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
         _float_tensor(out, 'out', 3, gate.dtype, dev)
         if out.shape != gate.shape:
             raise ValueError(f'out: expected {tuple(gate.shape)}, got {tuple(out.shape)}')
+        _apart('out', out, gate=gate, value=value, state=state, state_out=state_out)
     last = _lane_state(state_out, 'state_out', B, D, dev)
-    if last is None:
+    if last is not None:
+        same = state is not None and state.data_ptr() == last.data_ptr()
+        _apart('state_out', last, gate=gate, value=value, state=None if same else state)
+    else:
         last = gate.new_empty((B, D), dtype=torch.float32)
     if B == 0 or T == 0:
         if last is not state:
@@ -1502,6 +1519,7 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
         ldy = dst.stride(0)
         if M > 1 and ldy < N:
             raise ValueError('out: its rows overlap')
+        _apart('out', out, x=x, weight=weight, bias=bias)
     pre = x.new_empty((M, N)) if want_pre and act else None
     if M == 0:
         return out, pre

@@ -60,8 +60,8 @@ def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state
     Differentiable once, with respect to ``gate``, ``value`` and ``state``.  States and sums are
     fp32.  An infinity among the inputs leaves its channel's later states infinite or NaN.
 
-    ``out`` / ``state_out`` (not under autograd): where to write the two results;
-    ``state_out`` may be ``state`` itself.
+    ``out`` / ``state_out`` (not under autograd): where to write the two results, apart from the
+    inputs in memory; only ``state_out`` may be ``state`` itself.
 
     To capture a training step into a graph, drop eager results of the same leaves first: torch
     itself ends the process when a captured backward meets their gradient accumulators."""
@@ -105,7 +105,7 @@ def fused_linear(x, weight, bias=None, residual=None, activation='none', out=Non
     Sums are fp32, the result is rounded once; fp32 inputs are multiplied in fp32.
     Differentiable once, with respect to every tensor; for the backward pass the value in front
     of the activation is kept in x's type, as a layer's output would be.  ``out`` (not under
-    autograd): where to write the result.
+    autograd): where to write the result; it may be the residual, no other input.
 
     To capture a training step into a graph, drop eager results of the same leaves first: torch
     itself ends the process when a captured backward meets their gradient accumulators."""

@@ -170,6 +170,17 @@ def test_row_strides_and_offsets(K, N, dtype, act, gpu_device):
     R.check(one[None], ref1['y'], ref1['y_tol'], 'one vector')
 
 
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('M,K,N', [(200, 72, 40), (5, 300, 33), (3000, 64, 24), (600, 33, 130)])
+def test_residual_in_place(M, K, N, dtype, gpu_device):
+    import tempo_amd
+    t = _make(M, K, N, dtype, gpu_device, seed=8, residual=True)
+    want = tempo_amd.fused_linear(t['x'], t['weight'], t['bias'], t['residual'], 'gelu')
+    stream = t['residual'].clone()
+    got = tempo_amd.fused_linear(t['x'], t['weight'], t['bias'], stream, 'gelu', out=stream)
+    assert got is stream and torch.equal(got, want)
+
+
 def test_channels_last_map_is_read_in_place(gpu_device):
     import tempo_amd
     m = torch.randn(2, 24, 6, 10, device=gpu_device).contiguous(memory_format=torch.channels_last)
@@ -276,7 +287,9 @@ def test_refusals(gpu_device):
                 lambda: f(x.t().contiguous().t(), w), lambda: f(x, w[:0]),
                 lambda: f(x[:, :0], w[:, :0]), lambda: f(x, w, out=torch.empty(4, 6)),
                 lambda: f(x.view(2, 3, 8).transpose(0, 1), w),
-                lambda: f(x, w, out=torch.empty(4, device=gpu_device).expand(6, 4))):
+                lambda: f(x, w, out=torch.empty(4, device=gpu_device).expand(6, 4)),
+                lambda: f(x, w, out=x[:, 4:]), lambda: f(x[:4], w, out=w[:, :4]),
+                lambda: f(x, torch.ones(8, 8, device=gpu_device), out=x)):
         with pytest.raises(ValueError):
             bad()
     leaf = x.clone().requires_grad_(True)

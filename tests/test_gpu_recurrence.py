@@ -296,6 +296,7 @@ def test_refusals(gpu_device):
     gate, value = _inputs(2, 5, 6, torch.float32, gpu_device)
     state = torch.zeros(2, 6, device=gpu_device)
     lengths = torch.ones(2, dtype=torch.int32, device=gpu_device)
+    both, rows = torch.cat([gate, value], -1), torch.zeros(3, 6, device=gpu_device)
     for bad in (lambda: f(gate.cpu(), value), lambda: f(gate, value.half()),
                 lambda: f(gate.double(), value.double()), lambda: f(gate.long(), value.long()),
                 lambda: f(gate, value, state=state.half()),
@@ -311,7 +312,10 @@ def test_refusals(gpu_device):
                 lambda: f(gate, value, state=torch.zeros(6, 2, device=gpu_device).t()),
                 lambda: f(gate, value, lengths=lengths[:1]),
                 lambda: f(gate, value, out=gate[:1]),
-                lambda: f(gate, value, state_out=state[:1])):
+                lambda: f(gate, value, state_out=state[:1]),
+                lambda: f(gate, value, out=value), lambda: f(gate, value, out=gate),
+                lambda: f(both[..., :6], both[..., 6:], out=both[..., 3:9]),
+                lambda: f(gate, value, state=rows[:2], state_out=rows[1:])):
         with pytest.raises(ValueError):
             bad()
     leaf = gate.clone().requires_grad_(True)
