@@ -529,7 +529,9 @@ struct TinyGather {
 };
 
 // 128 x 128 of C per workgroup, 4 waves of 64 x 64; loads of the next 128 bytes of k fly under
-// the products of the present ones.
+// the products of the present ones.  4999 x 515 x 1021 in fp16: 22 us for each of the three
+// products (0.24 PFLOP/s; a third of that time is loads through registers, most of the rest the
+// latency of few steps in few tiles) and 11 us where two parts of k are joined.
 template <typename T, int AL, int BL, bool TINY>
 __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
   typedef Tile<T, AL, 128> TA;
@@ -622,7 +624,12 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
 // The same product where every 16-byte chunk of both operands is aligned and wholly inside or
 // outside of its row: tiles go from memory straight to LDS (buffer_load ... lds), so no
 // register holds data in flight and a workgroup can be 256 x 256, which halves what each
-// product reads from LDS.  Chunks outside an operand carry an offset beyond the buffer's
+// product reads from LDS.  16384 x 4096 x 4096 in bf16: 464 us bare (1.18 PFLOP/s; the library's
+// product 354 us), 523 us with a residual; what bounds it is the way from L2 to LDS -- on loads
+// that all miss memory the same loop runs at 2.1 PFLOP/s, on loads that hit L2 at 1.42 -- and at
+// short k the epilogue, which nothing overlaps (8192 x 4096 x 1024: 75 us bare, 117 with gelu and
+// the values kept for the backward pass).  128 x 256 tiles, two workgroups a compute unit, do
+// overlap it and lose more in the loop (600 us).  Chunks outside an operand carry an offset beyond the buffer's
 // range, for which the hardware writes zeros.  A chunk's place in LDS follows from its lane
 // (base + 16 lane), hence the lane picks the chunk that belongs to its place.
 
@@ -886,7 +893,9 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, ui
 // J <= 32 NJ, B small enough to stay in LDS: a workgroup lays B out in fragment order once and
 // its waves stream rows of A, 32 at a time, from memory right into the matrix units' operand
 // registers, the next kChunk steps ahead of the products.  Nothing but A's rows and the
-// result moves, at any alignment.
+// result moves, at any alignment: memory bounds it, 614400 x 64 x 256 in bf16 98 us (4.0 TB/s),
+// 153600 x 32 x 256 in fp32 57 us (3.5 TB/s with the values kept for the backward pass).  Twelve
+// waves a compute unit count for more than deeper loads: 126 us with eight.
 constexpr int kChunk = 8;  // steps in flight per wave: 32 rows x 256 bytes
 
 template <typename T>
@@ -1113,7 +1122,6 @@ __global__ __launch_bounds__(kFewWaves * 64) void few_kernel(const TileArgs a) {
 
 // --------------------------------------------------------------- gradient of z, bias gradient
 
-constexpr int kRowsPerBlock = 512;
 
 template <bool FULL, int V, typename Chunk>
 __device__ __forceinline__ void slopes(const Chunk& z, float (&d)[V], int act) {
@@ -1135,19 +1143,19 @@ __device__ __forceinline__ void slopes(const Chunk& z, float (&d)[V], int act) {
 // dz = g * act'(z) in the tensors' type (unless dz is NULL) and the sums of the unrounded
 // values over the workgroup's rows (right into db where one workgroup holds them all).  A thread
 // owns 16 bytes of columns, 8 threads side by side, four rows of each under way at a time: 8192 x
-// 4096 in bf16 54 us, 3.7 TB/s.
+// 4096 in bf16 50 us, 4.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long ldg, const T* pre,
                                                           T* dz, float* sums, T* db, long long M,
-                                                          int N, int act) {
+                                                          int N, int act, int rows) {
   constexpr bool FULL = sizeof(T) == 4;
   constexpr int V = 16 / sizeof(T), kWide = 8 * V, kRows = 4;
   typedef typename Pack<T, V>::type Chunk;
   __shared__ float s_sum[kWide][33];
   const int j = blockIdx.y * kWide + threadIdx.x % 8 * V;
   const int r = threadIdx.x / 8;
-  const long long first = (long long)blockIdx.x * kRowsPerBlock;
-  const long long stop = min(M, first + kRowsPerBlock);
+  const long long first = (long long)blockIdx.x * rows;
+  const long long stop = min(M, first + rows);
   const int n = max(0, min(V, N - j));
   float sum[V];
 #pragma unroll
@@ -1213,8 +1221,10 @@ __global__ __launch_bounds__(kThreads) void grad_bias_kernel(const float* sums, 
   __shared__ float s_sum[32][9];
   const int col = blockIdx.x * 8 + threadIdx.x % 8, r = threadIdx.x / 8;
   float sum = 0.f;
-  if (col < N)
+  if (col < N) {
+#pragma unroll 8
     for (long long b = r; b < blocks; b += 32) sum += sums[b * N + col];
+  }
   s_sum[r][threadIdx.x % 8] = sum;
   __syncthreads();
   if (threadIdx.x < 8 && col < N) {
@@ -1412,6 +1422,7 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
 }
 
 struct BackwardPlan {
+  int rows;  // of grad_z_kernel's workgroups
   long long dz_bytes, sum_bytes, scratch_bytes;
   long long total() const { return dz_bytes + sum_bytes + scratch_bytes; }
 };
@@ -1423,7 +1434,12 @@ bool plan_backward(long long M, int N, int K, int dtype, int act, BackwardPlan* 
   if (!product_bytes(M, K, N, K_ADJACENT, ROW_ADJACENT, dtype, &x) ||
       !product_bytes(N, K, M, ROW_ADJACENT, ROW_ADJACENT, dtype, &w)) return false;
   p->dz_bytes = act == NONE ? 0 : up16(M * N * (dtype == TEMPO_DTYPE_F32 ? 4 : 2));
-  p->sum_bytes = up16((M + kRowsPerBlock - 1) / kRowsPerBlock * N * 4);
+  // few sums to add up, but four workgroups for each compute unit where the matrix allows it
+  // (4999 x 515 in fp16: 32 us with 512 rows each, 12 with 128)
+  const long long groups = (N + 127) / 128;
+  p->rows = 512;
+  while (p->rows > 128 && (M + p->rows - 1) / p->rows * groups < 4 * kUnits) p->rows /= 2;
+  p->sum_bytes = up16((M + p->rows - 1) / p->rows * N * 4);
   p->scratch_bytes = up16(x > w ? x : w);
   return true;
 }
@@ -1449,12 +1465,12 @@ int backward_for(const BackwardPlan& p, const void* g, long long ldg, const void
   T* dz = act == NONE ? nullptr : (T*)ws;
   float* sums = db ? (float*)(ws + p.dz_bytes) : nullptr;
   float* scratch = (float*)(ws + p.dz_bytes + p.sum_bytes);
-  const long long blocks = (M + kRowsPerBlock - 1) / kRowsPerBlock;
+  const long long blocks = (M + p.rows - 1) / p.rows;
   if (dz || db) {
     constexpr int wide = 128 / sizeof(T);
     hipLaunchKernelGGL((grad_z_kernel<T>), dim3((unsigned)blocks, (N + wide - 1) / wide),
                        dim3(kThreads), 0, stream, (const T*)g, ldg, (const T*)pre, dz, sums,
-                       (T*)db, M, N, act);
+                       (T*)db, M, N, act, p.rows);
     if (db && blocks > 1)
       hipLaunchKernelGGL((grad_bias_kernel<T>), dim3((N + 7) / 8), dim3(kThreads), 0, stream,
                          sums, blocks, N, (T*)db);
