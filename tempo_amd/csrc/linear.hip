@@ -1315,7 +1315,9 @@ bool plan_product(long long I, long long J, long long K, int al, int bl, int dty
   p->tj = (uint32_t)tj;
   const long long depth = 128 / size;
   const long long steps = (K + depth - 1) / depth;
-  const long long fill = p->kernel == STREAM_256 ? kUnits : 2 * kUnits;  // workgroups at a time
+  // workgroups that keep the card busy: one a compute unit where it alone does (256 x 256 tiles,
+  // fp32, whose products take 16 times as long: 4096 x 1024 x 1024 trained 274 us, 294 with two)
+  const long long fill = p->kernel == STREAM_256 || size == 4 ? kUnits : 2 * kUnits;
   long long split = fill / (ti * tj);
   if (split > steps / 4) split = steps / 4;
   if (split < 1) split = 1;
