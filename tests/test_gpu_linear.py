@@ -83,7 +83,8 @@ def test_more_tiles_than_compute_units(shape, dtype, gpu_device):
 @pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize('shape', [(16411, 256, 32), (16384, 256, 64), (16400, 321, 17),
                                    (16385, 24, 40), (20001, 64, 100), (16411, 32, 256),
-                                   (16390, 520, 8), (16384, 1, 1), (16400, 130, 129)], ids=str)
+                                   (16390, 520, 8), (16384, 1, 1), (16400, 130, 129),
+                                   (2100, 504, 8), (2048, 248, 64), (2047, 64, 20)], ids=str)
 def test_many_rows_of_few_channels(shape, dtype, gpu_device):
     M, K, N = shape
     for i, act in enumerate(('none', ACTS[1 + (M + K + N) % 5])):

@@ -204,18 +204,45 @@ def test_gates_at_their_limits(T, D, gpu_device):
     assert float((h - 0.7).abs().max()) <= (1 + T / 32) * 2.0 ** -24
 
 
-def test_nan_stays_in_its_channel(gpu_device):
+@pytest.mark.parametrize('dtype', DTYPES[1:], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('T', [3, 2000])
+def test_gates_at_their_limits_in_16_bits(T, dtype, gpu_device):
     import tempo_amd
-    gate, value = _inputs(2, 300, 12, torch.float32, gpu_device)
+    gate, value = _inputs(2, T, 9, dtype, gpu_device, seed=21)
+    state, _ = _states(2, 9, gpu_device)
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    shut = torch.full_like(gate, float('-inf'))
+    shut[:, 1::3] = low
+    h, last = tempo_amd.gated_recurrence(shut, value, state=state)
+    assert torch.equal(last, state) and torch.equal(h, state.to(dtype)[:, None].expand_as(h))
+    for t, x in enumerate((float('inf'), high, float('-inf'), low, 100.0, -100.0)):
+        gate[:, t::11] = x
+    ref = R.recurrence(gate, value, state)
+    h, last = tempo_amd.gated_recurrence(gate, value, state=state)
+    R.check(h, ref['h'], ref['h_tol'], 'h')
+    R.check(last, ref['last'], ref['last_tol'], 'last')
+
+
+@pytest.mark.parametrize('T', [12, 300])
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+def test_nan_stays_in_its_channel(dtype, T, gpu_device):
+    import tempo_amd
+    gate, value = _inputs(2, T, 12, dtype, gpu_device)
     clean, _ = tempo_amd.gated_recurrence(gate, value)
-    value[1, 150, 3] = float('nan')
+    value[1, T // 2, 3] = float('nan')
     gate[0, 7, 5] = float('nan')
     h, _ = tempo_amd.gated_recurrence(gate, value)
     bad = torch.zeros_like(h, dtype=torch.bool)
-    bad[1, 150:, 3] = True
+    bad[1, T // 2:, 3] = True
     bad[0, 7:, 5] = True
     assert bool(h[bad].isnan().all())
     assert torch.equal(h[~bad], clean[~bad])
+    # backwards it reaches the steps in front of it, of its channel
+    grad = torch.ones_like(h)
+    _, _, g = _train(gpu_device, gate, value, None, None, grad, None)
+    for name in g:
+        other = [c for c in range(12) if c not in (3, 5)]
+        assert not bool(g[name][..., other].isnan().any())
 
 
 def test_gradients_are_the_differences(gpu_device):
