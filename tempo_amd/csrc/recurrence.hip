@@ -220,8 +220,11 @@ __device__ __forceinline__ void load_state(const float* p, const RecurrenceArgs&
 
 // ------------------------------------------------------------------------------- forward
 
-// kBatch steps of two streams; the last batch of a chunk holds its last step again in place of
-// those that are missing.  (Loading a batch ahead changed nothing: other waves fill the gaps.)
+// kBatch steps of two streams.  (Loading a batch ahead changed nothing: other waves fill the
+// gaps.)  Steps missing from a chunk's last batch are left out in 16 bits (31164 x 1 x 1072: 127
+// us, 169 with the last step loaded in their place); in fp32, where one step is more of the time
+// (102 against 106), that costs registers and with them a third of the waves (8 x 8192 x 1024: 345
+// against 333), so there they are the last step again.
 template <typename T, int V>
 struct Batch {
   typename Pack<T, V>::type a[kBatch], b[kBatch];
@@ -239,6 +242,7 @@ struct Batch {
     } else {
 #pragma unroll
       for (int q = 0; q < kBatch; ++q) {
+        if (sizeof(T) == 2 && i + q >= steps) break;
         const uint32_t t = min((uint32_t)q, steps - 1 - i);
         a[q] = fetch<FULL, V>(pa + t * sa, n);
         b[q] = fetch<FULL, V>(pb + t * sb, n);
