@@ -206,8 +206,8 @@ __device__ __forceinline__ u32x4 load16(const T* p, long long left) {
 //   K_ADJACENT    [row][k], 128 bytes: chunk c of row r at c ^ (r / 2 % 8), for two rows are all
 //                 banks (c ^ (r % 8): half of the LDS's cycles were conflicts);  64 bytes: four
 //                 rows are, c ^ (r / 4 % 4)
-//   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4) (32 rows: as it is, four
-//                 lines are all banks already);  fp32: as it is
+//   ROW_ADJACENT  [k][row], 16 bit: chunk c of line k at c ^ 4 (k % 4) (64 rows: two lines are all
+//                 banks, c ^ 4 (k / 2 % 2);  32: four are, as it is);  fp32: as it is
 template <typename T, int LAYOUT, int ROWS, int BYTES = 128>
 struct Tile {
   static constexpr int E = 16 / sizeof(T);
@@ -222,6 +222,8 @@ struct Tile {
       return BYTES == 128 ? c ^ (line / 2 & 7) : c ^ (line / 4 & 3);
     else if constexpr (sizeof(T) == 2 && ROWS >= 128)
       return c ^ (4 * (line & 3));
+    else if constexpr (sizeof(T) == 2 && ROWS == 64)
+      return c ^ (4 * (line / 2 & 1));
     else
       return c;
   }
@@ -389,13 +391,13 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long i, uint32_t 
 
 constexpr int kTogether = 4;  // rows of an epilogue that are under way at a time
 
-// A slab of sums in LDS (row i, 16-byte chunk c at c ^ (i % 32)) to memory: rows row0 .. row0 +
-// high - 1 of C, threads side by side along a row.
+// A slab of sums in LDS to memory: rows row0 .. row0 + high - 1 of C, threads side by side along
+// a row.  16-byte chunk c of row i lies at c ^ (i % 32), i % 16 where a row has 16.
 template <typename T, uint32_t QUADS, uint32_t THREADS>
 __device__ __forceinline__ void write_slab(const TileArgs& a, const char* lds, long long row0,
                                            uint32_t high, long long j0) {
   const uint32_t c = threadIdx.x % QUADS;
-  constexpr uint32_t kApart = THREADS / QUADS;
+  constexpr uint32_t kApart = THREADS / QUADS, kMask = QUADS < 32 ? QUADS - 1 : 31;
   const long long j = j0 + c * 4;
   if (j >= a.J) return;
   const int n = (int)min(4ll, a.J - j);
@@ -405,7 +407,7 @@ __device__ __forceinline__ void write_slab(const TileArgs& a, const char* lds, l
 #pragma unroll
     for (int r = 0; r < kTogether; ++r) {
       const uint32_t row = min(i + r * kApart, high - 1);
-      v[r] = *reinterpret_cast<const f32x4*>(lds + (row * QUADS + (c ^ (row & 31))) * 16);
+      v[r] = *reinterpret_cast<const f32x4*>(lds + (row * QUADS + (c ^ (row & kMask))) * 16);
     }
     if (a.e.partial) {
 #pragma unroll
@@ -443,9 +445,9 @@ __device__ __forceinline__ u32x4 shift_down(u32x4 r, uint32_t n) {
 // and inside the operand, without a branch: a chunk across the end of its row is loaded so that
 // it ends there and moved down afterwards, rows and k beyond the end are loaded from the last
 // ones, k beyond the end then set to 0.  Needs 16 bytes in the adjacent direction.
-template <typename T, int LAYOUT>
+template <typename T, int LAYOUT, int ROWS>
 struct Gather {
-  typedef Tile<T, LAYOUT, 128> Shape;
+  typedef Tile<T, LAYOUT, ROWS> Shape;
   static constexpr int E = Shape::E, kCount = Shape::kPerThread;
   const T* at[kCount];
   long long ld;
@@ -455,7 +457,7 @@ struct Gather {
 
   __device__ __forceinline__ Gather(const void* p, long long ld_, long long row0, long long rows) {
     ld = ld_;
-    edge = LAYOUT == ROW_ADJACENT && row0 + 128 > rows;
+    edge = LAYOUT == ROW_ADJACENT && row0 + ROWS > rows;
 #pragma unroll
     for (int n = 0; n < kCount; ++n) {
       const uint32_t q = n * kThreads + threadIdx.x;
@@ -511,9 +513,9 @@ struct Gather {
 };
 
 // The same for operands shorter than that, element by element
-template <typename T, int LAYOUT>
+template <typename T, int LAYOUT, int ROWS>
 struct TinyGather {
-  typedef Tile<T, LAYOUT, 128> Shape;
+  typedef Tile<T, LAYOUT, ROWS> Shape;
   const T* p;
   long long ld, row0, rows;
   __device__ __forceinline__ TinyGather(const void* p_, long long ld_, long long row0_,
@@ -528,32 +530,33 @@ struct TinyGather {
   }
 };
 
-// 128 x 128 of C per workgroup, 4 waves of 64 x 64; loads of the next 128 bytes of k fly under
-// the products of the present ones.  4999 x 515 x 1021 in fp16: 22 us for each of the three
+// 64 XI x 64 XJ of C per workgroup, 4 waves of a quarter each; loads of the next 128 bytes of k
+// fly under the products of the present ones.  4999 x 515 x 1021 in fp16: 22 us for each of the three
 // products (0.24 PFLOP/s; a third of that time is loads through registers, most of the rest the
 // latency of few steps in few tiles) and 11 us where two parts of k are joined.
-template <typename T, int AL, int BL, bool TINY>
+template <typename T, int AL, int BL, int XI, int XJ, bool TINY>
 __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
-  typedef Tile<T, AL, 128> TA;
-  typedef Tile<T, BL, 128> TB;
+  constexpr int kRows = 64 * XI, kCols = 64 * XJ;
+  typedef Tile<T, AL, kRows> TA;
+  typedef Tile<T, BL, kCols> TB;
   __shared__ __attribute__((aligned(16))) char lds[2][TA::kBytes + TB::kBytes];
   uint32_t i_tile, j_tile;
   tile_of(blockIdx.x, a.ti, a.tj, &i_tile, &j_tile);
-  const long long i0 = (long long)i_tile * 128, j0 = (long long)j_tile * 128;
+  const long long i0 = (long long)i_tile * kRows, j0 = (long long)j_tile * kCols;
   const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const uint32_t wi = wave / 2 * 64, wj = wave % 2 * 64;
+  const uint32_t wi = wave / 2 * (32 * XI), wj = wave % 2 * (32 * XJ);
   const uint32_t k_begin = blockIdx.y * (uint32_t)a.k_part, K = (uint32_t)a.K;
   const uint32_t k_end = min(K, k_begin + (uint32_t)a.k_part);
-  typedef typename std::conditional<TINY, TinyGather<T, AL>, Gather<T, AL>>::type GA;
-  typedef typename std::conditional<TINY, TinyGather<T, BL>, Gather<T, BL>>::type GB;
+  typedef typename std::conditional<TINY, TinyGather<T, AL, kRows>, Gather<T, AL, kRows>>::type GA;
+  typedef typename std::conditional<TINY, TinyGather<T, BL, kCols>, Gather<T, BL, kCols>>::type GB;
   const GA ga(a.a, a.lda, i0, a.I);
   const GB gb(a.b, a.ldb, j0, a.J);
 
-  f32x16 acc[2][2];
+  f32x16 acc[XI][XJ];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+  for (int x = 0; x < XI; ++x)
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+    for (int y = 0; y < XJ; ++y)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
 
@@ -572,22 +575,23 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
     }
     const char* la = lds[now];
     const char* lb = la + TA::kBytes;
-    u32x4 fa[2][2], fb[2][2];
+    u32x4 fa[2][XI], fb[2][XJ];
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      fa[0][x] = TA::fragment(la, wi + 32 * x, 0, lane);
-      fb[0][x] = TB::fragment(lb, wj + 32 * x, 0, lane);
-    }
+    for (int x = 0; x < XI; ++x) fa[0][x] = TA::fragment(la, wi + 32 * x, 0, lane);
+#pragma unroll
+    for (int y = 0; y < XJ; ++y) fb[0][y] = TB::fragment(lb, wj + 32 * y, 0, lane);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
+      for (int x = 0; x < XI; ++x) {
         if (s < 3) {  // the next step's operands arrive under this one's products
           fa[s + 1 & 1][x] = TA::fragment(la, wi + 32 * x, s + 1, lane);
-          fb[s + 1 & 1][x] = TB::fragment(lb, wj + 32 * x, s + 1, lane);
+#pragma unroll
+          for (int y = x * XJ / XI; y < (x + 1) * XJ / XI; ++y)
+            fb[s + 1 & 1][y] = TB::fragment(lb, wj + 32 * y, s + 1, lane);
         }
 #pragma unroll
-        for (int y = 0; y < 2; ++y)  // C^T: a lane holds 4 neighbouring j of one i
+        for (int y = 0; y < XJ; ++y)  // C^T: a lane holds 4 neighbouring j of one i
           acc[x][y] = Mfma<T>::run(fb[s & 1][y], fa[s & 1][x], acc[x][y]);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -599,24 +603,26 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
     __syncthreads();
   }
 
-  // The tile's sums pass through LDS (64 KB, the operands are done with): a wave holds columns
-  // of rows, memory wants rows.  16-byte chunk c of row i lies at c ^ (i % 32).
+  // The tile's sums pass through LDS (the operands are done with): a wave holds columns
+  // of rows, memory wants rows.  See write_slab for where they lie.
   char* lc = lds[0];
+  constexpr uint32_t kQuads = kCols / 4, kMask = kQuads < 32 ? kQuads - 1 : 31;
+  static_assert(sizeof(lds) >= kRows * kCols * 4, "the tile's sums fit");
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
+  for (int x = 0; x < XI; ++x) {
 #pragma unroll
-    for (int y = 0; y < 2; ++y) {
+    for (int y = 0; y < XJ; ++y) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const uint32_t i = wi + 32 * x + lane % 32, c = (wj + 32 * y + 8 * g) / 4 + lane / 32;
         const f32x4 v = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2],
                          acc[x][y][4 * g + 3]};
-        *reinterpret_cast<f32x4*>(lc + (i * 32 + (c ^ (i & 31))) * 16) = v;
+        *reinterpret_cast<f32x4*>(lc + (i * kQuads + (c ^ (i & kMask))) * 16) = v;
       }
     }
   }
   __syncthreads();
-  write_slab<T, 32, kThreads>(a, lc, i0, (uint32_t)min(128ll, a.I - i0), j0);
+  write_slab<T, kQuads, kThreads>(a, lc, i0, (uint32_t)min((long long)kRows, a.I - i0), j0);
 }
 
 // ---------------------------------------------------- tile kernel on aligned operands
@@ -824,6 +830,7 @@ __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a
   // sums through LDS as above, kSlab rows at a time
   constexpr uint32_t kFit = STAGES * kStage / (kCols * 4) / (XI * 32) * (XI * 32);
   constexpr uint32_t kSlab = kFit < kRows ? kFit : kRows, kQuads = kCols / 4;
+  constexpr uint32_t kMask = kQuads < 32 ? kQuads - 1 : 31;
   static_assert(kSlab > 0, "a wave's rows fit in LDS");
 #pragma unroll
   for (uint32_t slab = 0; slab < kRows; slab += kSlab) {
@@ -839,7 +846,7 @@ __global__ __launch_bounds__(WI* WJ * 64, 2) void stream_kernel(const TileArgs a
             const uint32_t q = (wj + 32 * y + 8 * g) / 4 + lane / 32;
             const f32x4 v = {acc[x][y][4 * g], acc[x][y][4 * g + 1], acc[x][y][4 * g + 2],
                              acc[x][y][4 * g + 3]};
-            *reinterpret_cast<f32x4*>(lds + (i * kQuads + (q ^ (i & 31))) * 16) = v;
+            *reinterpret_cast<f32x4*>(lds + (i * kQuads + (q ^ (i & kMask))) * 16) = v;
           }
         }
       }
@@ -890,12 +897,11 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const float* partial, ui
 
 // ------------------------------------------------------------------------ many rows, few columns
 //
-// J <= 32 NJ, B small enough to stay in LDS: a workgroup lays B out in fragment order once and
+// J <= 32, B small enough to stay in LDS: a workgroup lays B out in fragment order once and
 // its waves stream rows of A, 32 at a time, from memory right into the matrix units' operand
 // registers, the next kChunk steps ahead of the products.  Nothing but A's rows and the
-// result moves, at any alignment: memory bounds it, 614400 x 64 x 256 in bf16 98 us (4.0 TB/s),
-// 153600 x 32 x 256 in fp32 57 us (3.5 TB/s with the values kept for the backward pass).  Twelve
-// waves a compute unit count for more than deeper loads: 126 us with eight.
+// result moves, at any alignment: memory bounds it: 614400 x 32 x 256 in bf16 71 us
+// (5.0 TB/s), 153600 x 32 x 256 in fp32 38 us (4.7 TB/s).
 constexpr int kChunk = 8;  // steps in flight per wave: 32 rows x 256 bytes
 
 template <typename T>
@@ -905,20 +911,19 @@ struct ThinArgs {
   int b_layout;
 };
 
-template <typename T, int NJ>
+template <typename T>
 __global__ __launch_bounds__(kThreads, 3) void thin_kernel(const ThinArgs<T> args) {
   constexpr int E = 16 / sizeof(T), kStep = 2 * E;
   constexpr uint32_t kQuads = 8;
-  // rows of the epilogue under way at a time: what 168 registers hold without spills
-  constexpr int kThinTogether = NJ == 2 && sizeof(T) == 4 ? 1 : 2;
+  constexpr int kThinTogether = 2;  // rows of the epilogue under way at a time
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const TileArgs& a = args.t;
   const uint32_t lane = threadIdx.x % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const T* pb = (const T*)a.b;
-  for (uint32_t q = threadIdx.x; q < NJ * args.steps * 64; q += kThreads) {
-    const uint32_t l = q % 64, s = q / 64 % args.steps, jb = q / 64 / args.steps;
-    const long long j = jb * 32 + l % 32, k = (long long)s * kStep + l / 32 * E;
+  for (uint32_t q = threadIdx.x; q < args.steps * 64; q += kThreads) {
+    const uint32_t l = q % 64, s = q / 64;
+    const long long j = l % 32, k = (long long)s * kStep + l / 32 * E;
     u32x4 v = {0, 0, 0, 0};
     if (j < a.J) {
       if (args.b_layout == K_ADJACENT) {
@@ -933,17 +938,15 @@ __global__ __launch_bounds__(kThreads, 3) void thin_kernel(const ThinArgs<T> arg
     *reinterpret_cast<u32x4*>(lds + (size_t)q * 16) = v;
   }
   __syncthreads();
-  char* turn = lds + (size_t)NJ * args.steps * 1024 + wave * 4096;
+  char* turn = lds + (size_t)args.steps * 1024 + wave * 4096;
 
   const uint32_t chunks = (args.steps + kChunk - 1) / kChunk;
   const uint32_t stride = gridDim.x * (kThreads / 64);
   uint32_t block = blockIdx.x * (kThreads / 64) + wave, chunk = 0;
   if (block >= args.blocks) return;
-  f32x16 acc[NJ];
+  f32x16 acc;
 #pragma unroll
-  for (int y = 0; y < NJ; ++y)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[y][r] = 0.f;
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 
   auto fetch = [&](u32x4(&f)[kChunk], uint32_t blk, uint32_t chk) {
     const long long i = min((long long)blk * 32 + lane % 32, a.I - 1);
@@ -966,54 +969,47 @@ __global__ __launch_bounds__(kThreads, 3) void thin_kernel(const ThinArgs<T> arg
 #pragma unroll
     for (int s = 0; s < kChunk; ++s) {
       if (s0 + s < args.steps) {
-#pragma unroll
-        for (int y = 0; y < NJ; ++y) {
-          const u32x4 fb =
-              *reinterpret_cast<const u32x4*>(pf + ((size_t)y * args.steps + s) * 1024);
-          acc[y] = Mfma<T>::run(fb, f[s], acc[y]);
-        }
+        const u32x4 fb = *reinterpret_cast<const u32x4*>(pf + (size_t)s * 1024);
+        acc = Mfma<T>::run(fb, f[s], acc);
       }
     }
     if (chk + 1 < chunks) return;
     const long long left = a.I - (long long)blk * 32;
     const uint32_t high = (uint32_t)min(32ll, left);
 #pragma unroll
-    for (int y = 0; y < NJ; ++y) {
+    for (int g = 0; g < 4; ++g) {
+      const uint32_t i = lane % 32, q = 2 * g + lane / 32;
+      f32x4 v;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t i = lane % 32, q = 2 * g + lane / 32;
-        f32x4 v;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          v[r] = acc[y][4 * g + r];
-          acc[y][4 * g + r] = 0.f;
-        }
-        *reinterpret_cast<f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16) = v;
+      for (int r = 0; r < 4; ++r) {
+        v[r] = acc[4 * g + r];
+        acc[4 * g + r] = 0.f;
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      const uint32_t q = lane % kQuads;
-      const long long j = y * 32 + q * 4;
-      const int n = (int)min(4ll, a.J - j);
-      if (n > 0) {
-        constexpr uint32_t kApart = 64 / kQuads;
-#pragma unroll 1
-        for (uint32_t i = lane / kQuads; i < high; i += kThinTogether * kApart) {
-          f32x4 v[kThinTogether];
-#pragma unroll
-          for (int r = 0; r < kThinTogether; ++r) {
-            const uint32_t row = i + r * kApart;  // < 32, the block's rows
-            v[r] = *reinterpret_cast<const f32x4*>(
-                turn + (row * kQuads + (q ^ (row % kQuads))) * 16);
-          }
-          finish<T, kThinTogether>(a.e, (long long)blk * 32 + i, kApart, a.I, j, n, v);
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      *reinterpret_cast<f32x4*>(turn + (i * kQuads + (q ^ (i % kQuads))) * 16) = v;
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const uint32_t q = lane % kQuads;
+    const long long j = q * 4;
+    const int n = (int)min(4ll, a.J - j);
+    if (n > 0) {
+      constexpr uint32_t kApart = 64 / kQuads;
+#pragma unroll 1
+      for (uint32_t i = lane / kQuads; i < high; i += kThinTogether * kApart) {
+        f32x4 v[kThinTogether];
+#pragma unroll
+        for (int r = 0; r < kThinTogether; ++r) {
+          const uint32_t row = i + r * kApart;  // < 32, the block's rows
+          v[r] = *reinterpret_cast<const f32x4*>(
+              turn + (row * kQuads + (q ^ (row % kQuads))) * 16);
+        }
+        finish<T, kThinTogether>(a.e, (long long)blk * 32 + i, kApart, a.I, j, n, v);
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
   };
 
   u32x4 one[kChunk], two[kChunk];
@@ -1240,21 +1236,29 @@ constexpr int kUnits = 256;  // compute units to fill
 
 // Which kernel runs a product, by sizes and alignment alone.  Measured with the rule and with
 // the other side of it, in us:
-//   FEW    up to kFewRows rows, both operands with k adjacent (forward).  8 x 4096 x 4096 in bf16
-//          10 against 15 (split tiles), 64 rows 22 against 24; in fp32 53 against 50
-//   THIN   from kThinRows rows on, up to kThinColumns columns, A with k adjacent, B within half
-//          of the LDS.  65536 x 32 x 256 in fp32 22 against 42, 4096 rows 17 against 22;
-//          wider outputs lose (dx of 614400 x 32 x 256 in bf16, 256 columns: 115 against 167)
+//   FEW    up to kFewRows rows, both operands with k adjacent (forward), where the columns fill
+//          the card and their sums are short: see few_cost.  8 x 4096 x 4096 in bf16 9 against 12
+//          (tiles), 64 rows 21 against 16; 64 x 1000 x 1000 6 against 7; 16 x 512 x 4096 9 against
+//          6; 32 x 16384 x 4096 48 against 25, in fp32 110 against 78
+//   THIN   more than thin_rows rows, up to kThinColumns columns, A with k adjacent, B in LDS.
+//          153600 x 16 x 64 in bf16 7 against 10, 614400 x 32 x 256 71 against 74, 65536 rows 10
+//          against 8; 153600 x 32 x 256 in fp32 38 against 49, 32768 rows 15 against 14; with B
+//          at 78 KB (31 x 500 in fp32) 88 against 96, at 64 KB in 16 bits (15 x 768) 49 against
+//          38.  Twice the columns lost: 614400 x 64 x 256 in bf16 91 against 82, in fp32 299
+//          against 205
 //   STREAM_32x256  both operands aligned, A's rows adjacent, at most 32 of them (the weight's
 //          gradient of a thin layer).  153600 x 32 x 256 in fp32 44 against 91, in bf16 75
 //          against 71 of which memory takes 74
 //   STREAM_256     both aligned, 16 bits, a 256 x 256 tile for every compute unit.  4096 x 4096 x
-//          1024 (256 tiles) 40 against 50 with 128 x 128; 4096 x 2048 x 2048 (128) 64 against 46
-//   STREAM_128     both aligned;   TILE  anything
-enum Kernel { FEW, THIN, TILE, STREAM_32x256, STREAM_128, STREAM_256 };
+//          1024 (256 tiles) 40 against 50 with 128 x 128; 4096 x 2048 x 2048 (128) 64 against 46;
+//          not where its estimate is more than the smaller tiles': 153600 x 128 x 256 49 against 28
+//   STREAM  both aligned;   TILE  anything;  both in tiles of 64 or 128 rows and columns, whichever
+//          leave the compute units the least to do: see tile_shape
+enum Kernel { FEW, THIN, TILE, STREAM, STREAM_32x256, STREAM_256 };
 
 struct Product {
   Kernel kernel;
+  int xi, xj;  // tiles of 64 xi x 64 xj
   uint32_t ti, tj, split;
   long long k_part;
   long long bytes(long long I, long long J) const {
@@ -1263,17 +1267,17 @@ struct Product {
 };
 
 constexpr int kFewRows = 64;
-constexpr int kThinColumns = 64;
-constexpr long long kThinRows = 2048;
-constexpr uint32_t kThinLds = 81920;  // half a compute unit's: two workgroups share one
+constexpr int kThinColumns = 32;
 
-uint32_t thin_blocks(long long J) { return J <= 32 ? 1 : 2; }  // of 32 columns
+// three workgroups to a compute unit in 16 bits; fp32 is paid back with two as well
+uint32_t thin_room(int size) { return size == 4 ? 81920 : 49152; }
 
-uint32_t thin_lds(long long J, long long K, int size) {
-  const uint32_t nj = thin_blocks(J);
+long long thin_rows(int size) { return size == 4 ? 32768 : 65536; }
+
+uint32_t thin_lds(long long K, int size) {
   const long long steps = (K * size + 31) / 32;
-  const long long bytes = nj * steps * 1024 + 4 * 4096;
-  return bytes > kThinLds ? 0 : (uint32_t)bytes;
+  const long long bytes = steps * 1024 + 4 * 4096;
+  return bytes > thin_room(size) ? 0 : (uint32_t)bytes;
 }
 
 // An operand that stream_kernel can take: every 16-byte chunk aligned and not across an end,
@@ -1285,42 +1289,94 @@ bool streamable(const void* p, long long ld, int layout, long long rows, long lo
                               : rows % e == 0 && ld >= rows;
 }
 
-// K is split where the tiles alone leave compute units idle, into parts of at least four
-// steps (512 bytes of k).
+// How many parts k is cut into where the tiles alone leave compute units idle: workgroups that
+// keep the card busy are one a compute unit where it alone does (256 x 256 tiles, fp32, whose
+// products take 16 times as long: 4096 x 1024 x 1024 trained 274 us, 294 with two), else two; a
+// part has at least four steps (512 bytes of k).
+long long parts_of(long long tiles, long long steps, bool one) {
+  const long long split = min((one ? kUnits : 2 * kUnits) / tiles, steps / 4);
+  return split < 1 ? 1 : split;
+}
+
+// Tiles of 128 x 128 read each operand least often; smaller ones compute less that lies beyond the
+// matrix, spread better over the compute units and leave less of k to split.  An estimate in ns
+// of each, from what was measured, decides:
+//   - 64 x 64 products over 128 bytes of k take a compute unit 150 ns in 16 bits, as they come
+//     from L2, which 128 x 64 tiles ask 1.5 times as much for and 64 x 64 twice; in fp32 500 ns,
+//     the matrix units' time, and 15 or 30 % more
+//   - no less than the operands at memory's rate: each XCD reads its run of tiles for itself
+//   - split sums are written and read again and take one more launch
+// us in tiles of 128 x 128, 128 x 64, 64 x 128, 64 x 64 (what it picks in brackets):
+//   bf16  4096 x 1024 x 1024 33 [19] 19 20        128 x 4096 x 4096      27 21 21 [17]
+//         2048 x 2048 x 2048 42 [34] 34 38        5000 x 2000 x 2000     [71] 85 84 103
+//         256 x 256 x 153600 [63] 76 77 86        16384 x 192 x 768      26 [13] 15 14
+//   fp32  6066 x 1282 x 3076 571 [419] 477 457    1282 x 3076 x 6066     849 693 689 [577]
+//         161713 x 33 x 296  131 [70] 144 83      16384 x 192 x 768      58 53 55 [43]
+double tile_shape(long long I, long long J, long long K, int size, Product* p) {
+  const long long steps = (K * size + 127) / 128;
+  const double unit = size == 4 ? 500 : 150;
+  double best = 0;
+  for (int xi = 2; xi > 0; --xi) {
+    for (int xj = 2; xj > 0; --xj) {
+      const long long ti = (I + 64 * xi - 1) / (64 * xi), tj = (J + 64 * xj - 1) / (64 * xj);
+      const long long parts = parts_of(ti * tj, steps, size == 4);
+      const double more = 4 - xi - xj, area = xi * xj;
+      const double rounds = (double)((ti * tj * parts + kUnits - 1) / kUnits);
+      const double work = rounds * ((steps + parts - 1) / parts) * area * unit *
+                          (size == 4 ? 1 + .15 * more : 1 + .5 * more);
+      const long long run = (ti * tj + 7) / 8, high = min(min(run, ti), 8ll);
+      const long long across = min(tj, (run + high - 1) / high), down = (run + across - 1) / across;
+      const double read =
+          (double)min(ti * tj, 8ll) * 64 * (down * xi + across * xj) * K * size / 4800;
+      const double join = parts > 1 ? 5000 + (double)parts * I * J * 8 / 4800 : 0;
+      const double cost = (work > read ? work : read) + join;
+      if (xi + xj == 4 || cost < best) best = cost, p->xi = xi, p->xj = xj;
+    }
+  }
+  return best;
+}
+
+// few_kernel's time by the same measure: 16 columns a compute unit, a step's loads and products
+// one behind the other
+double few_cost(long long I, long long J, long long K, int size) {
+  const int blocks = I <= 16 ? 1 : I <= 32 ? 2 : 4;
+  const double rounds = (double)((J + 16 * kUnits - 1) / (16 * kUnits));
+  return rounds * ((K * size + 127) / 128) * (60 + (size == 4 ? 83 : 62) * blocks);
+}
+
 bool plan_product(long long I, long long J, long long K, int al, int bl, int dtype, bool direct,
                   Product* p) {
   const int size = dtype == TEMPO_DTYPE_F32 ? 4 : 2;
   p->split = 1;
   p->k_part = K;
-  if (al == K_ADJACENT && bl == K_ADJACENT && I <= kFewRows) {
+  const double cost = tile_shape(I, J, K, size, p);
+  if (al == K_ADJACENT && bl == K_ADJACENT && I <= kFewRows && few_cost(I, J, K, size) <= cost) {
     p->kernel = FEW;
     return true;
   }
-  if (al == K_ADJACENT && J <= kThinColumns && I >= kThinRows && thin_lds(J, K, size)) {
+  if (al == K_ADJACENT && J <= kThinColumns && I > thin_rows(size) && thin_lds(K, size)) {
     p->kernel = THIN;
     return true;
   }
-  long long high = 128, wide = 128;
-  p->kernel = direct ? STREAM_128 : TILE;
+  const long long depth = 128 / size;
+  const long long steps = (K + depth - 1) / depth;
+  p->kernel = direct ? STREAM : TILE;
+  long long high = 64 * p->xi, wide = 64 * p->xj;
   if (direct && al == ROW_ADJACENT && I <= 32) {
     p->kernel = STREAM_32x256;
     high = 32, wide = 256;
-  } else if (direct && size == 2 && (I + 255) / 256 * ((J + 255) / 256) >= kUnits) {
-    p->kernel = STREAM_256;
-    high = wide = 256;
+  } else if (direct && size == 2) {
+    const long long tiles = (I + 255) / 256 * ((J + 255) / 256);
+    if (tiles >= kUnits && (tiles + kUnits - 1) / kUnits * (double)steps * 16 * 120 <= cost) {
+      p->kernel = STREAM_256;
+      high = wide = 256;
+    }
   }
   const long long ti = (I + high - 1) / high, tj = (J + wide - 1) / wide;
   if (ti > 0x3fffffff / tj) return false;
   p->ti = (uint32_t)ti;
   p->tj = (uint32_t)tj;
-  const long long depth = 128 / size;
-  const long long steps = (K + depth - 1) / depth;
-  // workgroups that keep the card busy: one a compute unit where it alone does (256 x 256 tiles,
-  // fp32, whose products take 16 times as long: 4096 x 1024 x 1024 trained 274 us, 294 with two)
-  const long long fill = p->kernel == STREAM_256 || size == 4 ? kUnits : 2 * kUnits;
-  long long split = fill / (ti * tj);
-  if (split > steps / 4) split = steps / 4;
-  if (split < 1) split = 1;
+  const long long split = parts_of(ti * tj, steps, p->kernel == STREAM_256 || size == 4);
   const long long part = (steps + split - 1) / split;
   p->k_part = part * depth;
   p->split = (uint32_t)((steps + part - 1) / part);
@@ -1353,13 +1409,6 @@ int run_few(const TileArgs& t, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-template <typename T, int NJ>
-void launch_thin(const ThinArgs<T>& a, uint32_t lds, hipStream_t stream) {
-  const uint32_t groups = (a.blocks + 3) / 4;
-  const dim3 grid(groups < 3 * kUnits ? groups : 3 * kUnits);
-  hipLaunchKernelGGL((thin_kernel<T, NJ>), grid, dim3(kThreads), lds, stream, a);
-}
-
 template <typename T>
 int run_thin(const TileArgs& t, int b_layout, hipStream_t stream) {
   ThinArgs<T> a = {};
@@ -1367,10 +1416,23 @@ int run_thin(const TileArgs& t, int b_layout, hipStream_t stream) {
   a.blocks = (uint32_t)((t.I + 31) / 32);
   a.steps = (uint32_t)((t.K * (long long)sizeof(T) + 31) / 32);
   a.b_layout = b_layout;
-  const uint32_t lds = thin_lds(t.J, t.K, sizeof(T));
-  if (thin_blocks(t.J) == 1) launch_thin<T, 1>(a, lds, stream);
-  else launch_thin<T, 2>(a, lds, stream);
+  const uint32_t groups = (a.blocks + 3) / 4;
+  const dim3 grid(groups < 3 * kUnits ? groups : 3 * kUnits);
+  hipLaunchKernelGGL((thin_kernel<T>), grid, dim3(kThreads), thin_lds(t.K, sizeof(T)), stream, a);
   return (int)hipGetLastError();
+}
+
+template <typename T, int AL, int BL, int XI, int XJ>
+void launch_tile(const Product& p, const TileArgs& t, bool tiny, hipStream_t stream) {
+  const dim3 grid(p.ti * p.tj, p.split);
+  if (p.kernel == STREAM)
+    hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, XI, XJ, 64, 4>), grid, dim3(256), 0, stream,
+                       t);
+  else if (tiny)
+    hipLaunchKernelGGL((tile_kernel<T, AL, BL, XI, XJ, true>), grid, dim3(kThreads), 0, stream, t);
+  else
+    hipLaunchKernelGGL((tile_kernel<T, AL, BL, XI, XJ, false>), grid, dim3(kThreads), 0, stream,
+                       t);
 }
 
 template <typename T, int AL, int BL>
@@ -1394,15 +1456,14 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
   if constexpr (AL == K_ADJACENT) {
     if (p.kernel == THIN) return run_thin<T>(t, BL, stream);
   }
-  if (p.kernel == TILE) {
+  if (p.kernel == TILE || p.kernel == STREAM) {
     constexpr int e = 16 / sizeof(T);
-    if ((AL == K_ADJACENT ? K : I) < e || (BL == K_ADJACENT ? K : J) < e)
-      hipLaunchKernelGGL((tile_kernel<T, AL, BL, true>), grid, dim3(kThreads), 0, stream, t);
-    else
-      hipLaunchKernelGGL((tile_kernel<T, AL, BL, false>), grid, dim3(kThreads), 0, stream, t);
+    const bool tiny = (AL == K_ADJACENT ? K : I) < e || (BL == K_ADJACENT ? K : J) < e;
+    if (p.xi == 2 && p.xj == 2) launch_tile<T, AL, BL, 2, 2>(p, t, tiny, stream);
+    else if (p.xi == 2) launch_tile<T, AL, BL, 2, 1>(p, t, tiny, stream);
+    else if (p.xj == 2) launch_tile<T, AL, BL, 1, 2>(p, t, tiny, stream);
+    else launch_tile<T, AL, BL, 1, 1>(p, t, tiny, stream);
   }
-  if (p.kernel == STREAM_128)
-    hipLaunchKernelGGL((stream_kernel<T, AL, BL, 2, 2, 2, 2, 64, 4>), grid, dim3(256), 0, stream, t);
   if constexpr (AL == ROW_ADJACENT) {
     if (p.kernel == STREAM_32x256)
       hipLaunchKernelGGL((stream_kernel<T, AL, BL, 1, 4, 1, 2, 128, 2>), grid, dim3(256), 0, stream, t);

@@ -80,6 +80,19 @@ def test_more_tiles_than_compute_units(shape, dtype, gpu_device):
     _check_grads(_make(M, K, N, dtype, gpu_device, seed=4, residual=True, grad=True), 'silu')
 
 
+# products whose tiles are 64 or 128 rows by 64 or 128 columns, each in all three operand orders
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', [(70, 72, 72), (67, 65, 71), (4000, 16, 520), (2000, 72, 1000),
+                                   (2003, 71, 1001), (4000, 33, 1000), (4000, 520, 264),
+                                   (2000, 520, 1000), (180, 520, 4000), (180, 65, 8001),
+                                   (180, 130, 20000), (3999, 521, 1001), (4000, 520, 1000)],
+                         ids=str)
+def test_tile_shapes(shape, dtype, gpu_device):
+    M, K, N = shape
+    act = ACTS[(M + K + N) % 6]
+    _check_grads(_make(M, K, N, dtype, gpu_device, seed=7, residual=True, grad=True), act)
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
 @pytest.mark.parametrize('shape', [(16411, 256, 32), (16384, 256, 64), (16400, 321, 17),
                                    (16385, 24, 40), (20001, 64, 100), (16411, 32, 256),
@@ -90,6 +103,30 @@ def test_many_rows_of_few_channels(shape, dtype, gpu_device):
     for i, act in enumerate(('none', ACTS[1 + (M + K + N) % 5])):
         _check_grads(_make(M, K, N, dtype, gpu_device, seed=5 + i, bias=i == 0, residual=i == 1,
                            grad=True), act, f'{act} ')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', [(65539, 256, 32), (65537, 256, 64), (66000, 221, 17),
+                                   (65600, 24, 40), (65540, 32, 256), (65537, 1, 1),
+                                   (65536, 64, 33), (65541, 512, 8), (65541, 513, 8),
+                                   (65538, 257, 5), (32771, 63, 31), (32769, 31, 63)], ids=str)
+def test_more_rows_of_few_channels(shape, dtype, gpu_device):
+    M, K, N = shape
+    for i, act in enumerate(('none', ACTS[1 + (M + K + N) % 5])):
+        _check_grads(_make(M, K, N, dtype, gpu_device, seed=9 + i, bias=i == 0, residual=i == 1,
+                           grad=True), act, f'{act} ')
+
+
+# either kernel for up to 64 rows: the sums long and the columns few, the other way round, both
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('M', [1, 8, 16, 17, 31, 33, 48, 64])
+def test_few_rows_of_many_columns(M, dtype, gpu_device):
+    import tempo_amd
+    for K, N in ((256, 300), (1000, 1000), (1029, 999), (4096, 520), (515, 8200)):
+        t = _make(M, K, N, dtype, gpu_device, seed=8, residual=True)
+        ref = R.linear(t['x'], t['weight'], t['bias'], t['residual'], 'gelu')
+        y = tempo_amd.fused_linear(t['x'], t['weight'], t['bias'], t['residual'], 'gelu')
+        R.check(y, ref['y'], ref['y_tol'], f'y, {K} x {N}')
 
 
 @pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
