@@ -1138,18 +1138,18 @@ __device__ __forceinline__ void slopes(const Chunk& z, float (&d)[V], int act) {
 
 // dz = g * act'(z) in the tensors' type (unless dz is NULL) and the sums of the unrounded
 // values over the workgroup's rows (right into db where one workgroup holds them all).  A thread
-// owns 16 bytes of columns, 8 threads side by side, four rows of each under way at a time: 8192 x
-// 4096 in bf16 50 us, 4.0 TB/s.
-template <typename T>
+// owns 16 bytes of columns, WIDE threads side by side, four rows of each under way at a time: 8192
+// x 4096 in bf16 39 us, 5.2 TB/s.
+template <typename T, int WIDE>
 __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long ldg, const T* pre,
                                                           T* dz, float* sums, T* db, long long M,
                                                           int N, int act, int rows) {
   constexpr bool FULL = sizeof(T) == 4;
-  constexpr int V = 16 / sizeof(T), kWide = 8 * V, kRows = 4;
+  constexpr int V = 16 / sizeof(T), kWide = WIDE * V, kHigh = kThreads / WIDE, kRows = 4;
   typedef typename Pack<T, V>::type Chunk;
-  __shared__ float s_sum[kWide][33];
-  const int j = blockIdx.y * kWide + threadIdx.x % 8 * V;
-  const int r = threadIdx.x / 8;
+  __shared__ float s_sum[kWide][kHigh + 1];
+  const int j = blockIdx.y * kWide + threadIdx.x % WIDE * V;
+  const int r = threadIdx.x / WIDE;
   const long long first = (long long)blockIdx.x * rows;
   const long long stop = min(M, first + rows);
   const int n = max(0, min(V, N - j));
@@ -1157,11 +1157,11 @@ __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long 
 #pragma unroll
   for (int q = 0; q < V; ++q) sum[q] = 0.f;
   if (n > 0) {
-    for (long long i0 = first + r; i0 < stop; i0 += 32 * kRows) {
+    for (long long i0 = first + r; i0 < stop; i0 += kHigh * kRows) {
       Chunk gv[kRows], zv[kRows];
 #pragma unroll
       for (int x = 0; x < kRows; ++x) {
-        const long long i = min(i0 + 32 * x, stop - 1);
+        const long long i = min(i0 + kHigh * x, stop - 1);
         if (n == V) {
           gv[x] = *reinterpret_cast<const Chunk*>(g + i * ldg + j);
           if (pre) zv[x] = *reinterpret_cast<const Chunk*>(pre + i * N + j);
@@ -1175,7 +1175,7 @@ __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long 
       }
 #pragma unroll
       for (int x = 0; x < kRows; ++x) {
-        const long long i = i0 + 32 * x;
+        const long long i = i0 + kHigh * x;
         if (i >= stop) continue;
         float d[V];
         if (pre) slopes<FULL, V>(zv[x], d, act);
@@ -1199,12 +1199,12 @@ __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long 
   }
   if (!sums) return;
 #pragma unroll
-  for (int q = 0; q < V; ++q) s_sum[threadIdx.x % 8 * V + q][r] = sum[q];
+  for (int q = 0; q < V; ++q) s_sum[threadIdx.x % WIDE * V + q][r] = sum[q];
   __syncthreads();
-  if (threadIdx.x < kWide) {
+  for (int c = threadIdx.x; c < kWide; c += kThreads) {
     float total = 0.f;
-    for (int k = 0; k < 32; ++k) total += s_sum[threadIdx.x][k];
-    const int col = blockIdx.y * kWide + threadIdx.x;
+    for (int k = 0; k < kHigh; ++k) total += s_sum[c][k];
+    const int col = blockIdx.y * kWide + c;
     if (col < N && gridDim.x == 1) db[col] = (T)total;
     else if (col < N) sums[(long long)blockIdx.x * N + col] = total;
   }
@@ -1485,7 +1485,7 @@ int run_product(const void* a, long long lda, const void* b, long long ldb, long
 }
 
 struct BackwardPlan {
-  int rows;  // of grad_z_kernel's workgroups
+  int wide, rows;  // threads along a row and rows of grad_z_kernel's workgroups
   long long dz_bytes, sum_bytes, scratch_bytes;
   long long total() const { return dz_bytes + sum_bytes + scratch_bytes; }
 };
@@ -1497,11 +1497,23 @@ bool plan_backward(long long M, int N, int K, int dtype, int act, BackwardPlan* 
   if (!product_bytes(M, K, N, K_ADJACENT, ROW_ADJACENT, dtype, &x) ||
       !product_bytes(N, K, M, ROW_ADJACENT, ROW_ADJACENT, dtype, &w)) return false;
   p->dz_bytes = act == NONE ? 0 : up16(M * N * (dtype == TEMPO_DTYPE_F32 ? 4 : 2));
+  // A row's pieces that end inside a 128-byte line are written to memory twice, so a workgroup
+  // holds whole rows where it can (325353 x 280 in bf16: 126 us with 64 threads a row, 172 with
+  // 32, 207 with 8), but no idle threads where pieces end with lines (200000 x 96 in fp32: 64 us
+  // with 32, 55 with 8).  Beyond 64 threads a row, 32: 8192 x 4096 in bf16 40 us, 48 with 8, 44
+  // with 64.
+  const int size = dtype == TEMPO_DTYPE_F32 ? 4 : 2;
+  const int chunks = (N * size + 15) / 16;
+  p->wide = chunks <= 8 ? 8 : chunks <= 16 ? 16 : chunks <= 32 || chunks > 64 ? 32 : 64;
+  while (N * size % 128 == 0 && chunks % p->wide) p->wide /= 2;
+  // one workgroup for all rows needs no second launch (64 x 4096 in fp16: 4 us against 7)
+  if (M <= 128) p->wide = 8;
   // few sums to add up, but four workgroups for each compute unit where the matrix allows it
-  // (4999 x 515 in fp16: 32 us with 512 rows each, 12 with 128)
-  const long long groups = (N + 127) / 128;
+  // (5000 x 515 in fp16: 31 us with 128 rows each, 13 with 32)
+  const long long groups = (chunks + p->wide - 1) / p->wide;
   p->rows = 512;
-  while (p->rows > 128 && (M + p->rows - 1) / p->rows * groups < 4 * kUnits) p->rows /= 2;
+  while (p->rows > 1024 / p->wide && (M + p->rows - 1) / p->rows * groups < 4 * kUnits)
+    p->rows /= 2;
   p->sum_bytes = up16((M + p->rows - 1) / p->rows * N * 4);
   p->scratch_bytes = up16(x > w ? x : w);
   return true;
@@ -1530,8 +1542,12 @@ int backward_for(const BackwardPlan& p, const void* g, long long ldg, const void
   float* scratch = (float*)(ws + p.dz_bytes + p.sum_bytes);
   const long long blocks = (M + p.rows - 1) / p.rows;
   if (dz || db) {
-    constexpr int wide = 128 / sizeof(T);
-    hipLaunchKernelGGL((grad_z_kernel<T>), dim3((unsigned)blocks, (N + wide - 1) / wide),
+    constexpr int V = 16 / sizeof(T);
+    auto kernel = p.wide == 8    ? grad_z_kernel<T, 8>
+                  : p.wide == 16 ? grad_z_kernel<T, 16>
+                  : p.wide == 32 ? grad_z_kernel<T, 32>
+                                 : grad_z_kernel<T, 64>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (N + p.wide * V - 1) / (p.wide * V)),
                        dim3(kThreads), 0, stream, (const T*)g, ldg, (const T*)pre, dz, sums,
                        (T*)db, M, N, act, p.rows);
     if (db && blocks > 1)
