@@ -531,9 +531,9 @@ struct TinyGather {
 };
 
 // 64 XI x 64 XJ of C per workgroup, 4 waves of a quarter each; loads of the next 128 bytes of k
-// fly under the products of the present ones.  4999 x 515 x 1021 in fp16: 22 us for each of the three
-// products (0.24 PFLOP/s; a third of that time is loads through registers, most of the rest the
-// latency of few steps in few tiles) and 11 us where two parts of k are joined.
+// fly under the products of the present ones.  4999 x 515 x 1021 in fp16 and its gradients: 33,
+// 23 and 22 us (0.16 to 0.24 PFLOP/s; a third of that time is loads through registers, most of the
+// rest the latency of few steps in few tiles) and 7 us where parts of k are joined.
 template <typename T, int AL, int BL, int XI, int XJ, bool TINY>
 __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
   constexpr int kRows = 64 * XI, kCols = 64 * XJ;
