@@ -1373,7 +1373,7 @@ bool plan_product(long long I, long long J, long long K, int al, int bl, int dty
     }
   }
   const long long ti = (I + high - 1) / high, tj = (J + wide - 1) / wide;
-  if (ti > 0x3fffffff / tj) return false;
+  if (ti > 0xffffff / tj) return false;  // a grid's threads are counted in 32 bits
   p->ti = (uint32_t)ti;
   p->tj = (uint32_t)tj;
   const long long split = parts_of(ti * tj, steps, p->kernel == STREAM_256 || size == 4);

@@ -112,3 +112,14 @@ def test_linear_workspace():
     assert ws(1, 1, 1, 0, 9, 0) == -5 and ws(1, 1 << 21, 1, 0, 0, 0) == -4
     assert ws(16384, 4096, 4096, 2, 0, 0) == 0  # tiles enough: the sum is not split
     assert ws(8192, 4096, 1024, 2, 3, 1) >= 8192 * 4096 * 2  # dz
+
+
+def test_linear_grid_limit():
+    """A product of more tiles than a launch can hold is refused by size, one below it is not."""
+    workspace = _lib.load().tempo_linear_workspace
+    for dtype in (0, 1, 2):
+        assert workspace((1 << 31) - 1, 100, 8, dtype, 0, 0) == -4   # 2^24 tiles of 128 rows
+        assert workspace((1 << 31) - 1, 100, 8, dtype, 0, 1) > 0     # 8 columns: a fixed grid
+        assert workspace((1 << 31) - 1, 8, 100, dtype, 0, 0) == 0
+        assert workspace((1 << 31) - 1, 8, 100, dtype, 0, 1) == -4   # dx has 100
+        assert workspace(1 << 30, 100, 8, dtype, 0, 0) == 0          # 2^23
