@@ -122,18 +122,24 @@ __device__ __forceinline__ float slope(float z, int act) {
   }
 }
 
-// z in the tensors' type for the backward pass: relu asks for its sign, which an fp16
-// underflow would lose
+// z in the tensors' type for the backward pass.  relu asks for its sign, which an fp16 underflow
+// would lose; silu and gelu for a finite z to stay finite, for their slopes at an infinity are
+// infinity times 0.  Beyond the type's range they are what they are at its end.
 template <typename T>
-__device__ __forceinline__ T keep_sign(float z) {
-  T r = (T)z;
+__device__ __forceinline__ T keep_z(float z) {
   if constexpr (sizeof(T) == 2) {
+    const float most = std::is_same<T, _Float16>::value ? 65504.f : 0x1.fep127f;
+    const float inside = __builtin_amdgcn_fmed3f(z, -most, most);
+    const T r = (T)(fabsf(z) <= 0x1.fffffep127f ? inside : z);  // infinities and NaN stay
     if (z > 0.f && (float)r == 0.f) {
-      const uint16_t least = 1;
-      __builtin_memcpy(&r, &least, 2);
+      T least;
+      const uint16_t one = 1;
+      __builtin_memcpy(&least, &one, 2);
+      return least;
     }
+    return r;
   }
-  return r;
+  return (T)z;
 }
 
 // ------------------------------------------------------------------------------ tile kernel
@@ -355,7 +361,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, long long i, uint32_t 
       T* p = (T*)e.pre + (i + r * apart) * e.ldp + j;
       V4 kept;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) kept[q] = keep_sign<T>(z[r][q]);
+      for (int q = 0; q < 4; ++q) kept[q] = keep_z<T>(z[r][q]);
       if (n == 4) {
         *reinterpret_cast<V4*>(p) = kept;
       } else {

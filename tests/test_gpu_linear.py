@@ -420,3 +420,35 @@ def test_strides_beyond_32_bits(which, gpu_device):
     assert torch.equal(y, want_y)
     for k in want:
         assert torch.equal(g[k], want[k]), k
+
+
+@pytest.mark.parametrize('act', ACTS)
+def test_gradients_where_z_leaves_the_type(act, gpu_device):
+    """z beyond fp16's (bf16's) range is finite in the forward pass, and the slopes there are the
+    limits: nothing but zeros and ones, in dx, dW and db."""
+    import tempo_amd
+    up, down = {'none': (1, 1), 'relu': (1, 0), 'silu': (1, 0), 'gelu': (1, 0)}.get(act, (0, 0))
+    x = torch.tensor([[-300.0], [300.0], [0.0]], dtype=torch.float16, device=gpu_device)
+    t = {'x': x, 'weight': torch.full((1, 1), 300.0, dtype=torch.float16, device=gpu_device),
+         'bias': torch.zeros(1, dtype=torch.float16, device=gpu_device),
+         # z = -90000 and 90000: y fits fp16 again
+         'residual': x.new_tensor([[60000.0], [-60000.0], [0.0]]),
+         'grad': x.new_tensor([[1.0], [1.0], [0.0]])}
+    y, g = _train(t, act)
+    assert bool(torch.isfinite(y).all())
+    assert g['x'].flatten().tolist() == [300.0 * down, 300.0 * up, 0.0]
+    assert g['weight'].item() == 300.0 * (up - down) and g['bias'].item() == up + down
+    # one half step of bf16 beyond its largest value, still finite in fp32
+    x = torch.tensor([[-2.0 ** 64, -2.0 ** 60], [2.0 ** 64, 2.0 ** 60]], device=gpu_device)
+    w = torch.tensor([[2.0 ** 64 * (1 - 2.0 ** -8), 2.0 ** 59]], device=gpu_device)
+    t = {'x': x.bfloat16(), 'weight': w.bfloat16(), 'bias': None, 'residual': None,
+         'grad': x.new_ones(2, 1).bfloat16()}
+    assert torch.equal(t['x'].float(), x) and torch.equal(t['weight'].float(), w)
+    _, g = _train(t, act)
+    assert torch.equal(g['x'].float(), torch.cat([w * down, w * up]))
+    assert torch.equal(g['weight'].float(), x[:1] * down + x[1:] * up)
+    # an infinity among the inputs is not hidden
+    x = torch.tensor([[float('inf')], [float('nan')]], dtype=torch.float16, device=gpu_device)
+    y = tempo_amd.fused_linear(x, x.new_ones(1, 1), activation=act)
+    assert y[0].item() == {'sigmoid': 1.0, 'tanh': 1.0}.get(act, float('inf'))
+    assert bool(y[1].isnan())
