@@ -5,6 +5,7 @@ arithmetic happens in ``csrc/tempo_unproject.hip``.  All entry points require
 CUDA/HIP tensors and raise otherwise -- there is no CPU path.
 """
 import ctypes
+import math
 
 import torch
 
@@ -1302,16 +1303,27 @@ def _strided(t):
 
 
 def _apart(name, out, **inputs):
-    """Results are written while inputs are still read: they must not share memory."""
-    def ends(t):
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    """Results are written while inputs are still read: they must not share memory.  Channels
+    next to each other in the same rows do not: modulo a distance that divides all of their
+    rows' distances, each is one piece."""
+    def place(t):
+        size = t.element_size()
+        apart = [s * size for n, s in zip(t.shape[:-1], t.stride()) if n > 1]
+        width = t.shape[-1] * size
+        return t.data_ptr(), sum((n - 1) * s for n, s in zip(t.shape, t.stride())) * size + size, \
+            apart, width
     if not out.numel():
         return
-    low, high = ends(out)
+    low, high, apart, width = place(out)
     for other, t in inputs.items():
-        if t is not None and t.numel() and ends(t)[0] < high and low < ends(t)[1]:
-            raise ValueError(f'{name}: shares memory with {other}')
+        if t is None or not t.numel():
+            continue
+        low2, high2, apart2, width2 = place(t)
+        if low2 < low + high and low < low2 + high2:
+            by = math.gcd(*apart, *apart2)
+            gap = (low2 - low) % by if by else 0
+            if not (gap >= width and gap + width2 <= by):
+                raise ValueError(f'{name}: shares memory with {other}')
 
 
 def _like_time_order(t, channels):
@@ -1519,7 +1531,8 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
         ldy = dst.stride(0)
         if M > 1 and ldy < N:
             raise ValueError('out: its rows overlap')
-        _apart('out', out, x=x, weight=weight, bias=bias)
+        same = res is not None and res.data_ptr() == dst.data_ptr() and (M == 1 or ldr == ldy)
+        _apart('out', out, x=x, weight=weight, bias=bias, residual=None if same else residual)
     pre = x.new_empty((M, N)) if want_pre and act else None
     if M == 0:
         return out, pre

@@ -452,3 +452,40 @@ def test_gradients_where_z_leaves_the_type(act, gpu_device):
     y = tempo_amd.fused_linear(x, x.new_ones(1, 1), activation=act)
     assert y[0].item() == {'sigmoid': 1.0, 'tanh': 1.0}.get(act, float('inf'))
     assert bool(y[1].isnan())
+
+
+def test_out_and_residual_overlap(gpu_device):
+    """A residual that is read by one workgroup after another one wrote the result over it is
+    refused: shifted by a row or a channel, another distance between rows, rows that coincide.
+    The same memory in the same order is not."""
+    import tempo_amd
+    t = _make(6, 8, 4, torch.float32, gpu_device)
+    buf = torch.zeros(80, device=gpu_device)
+    rows, wide = buf[:28].view(7, 4), buf[:48].view(6, 8)
+
+    def call(residual, out, x=t['x']):
+        return tempo_amd.fused_linear(x, t['weight'], t['bias'], residual, 'relu', out=out)
+
+    for residual, out in ((rows[:6], rows[1:]), (rows[1:], rows[:6]), (rows[:6], wide[:, :4]),
+                          (wide[:, :4], rows[:6]), (wide[:, :4], wide[:, 1:5]),
+                          (rows[:1].expand(6, 4), rows[:6])):
+        with pytest.raises(ValueError, match='shares memory with residual'):
+            call(residual, out)
+    want = call(None, None) + 1
+    wide[:, :4] = 1  # next to each other in the same rows
+    call(wide[:, :4], wide[:, 4:])
+    assert torch.equal(wide[:, 4:], want) and bool((wide[:, :4] == 1).all())
+    for out in (rows[:6], wide[:, :4]):
+        out.fill_(1)
+        assert call(out.view_as(out), out) is out and torch.equal(out, want)
+    out = buf[:4].view(1, 4)  # one row: its distance to the next one means nothing
+    out.fill_(1)
+    call(torch.as_strided(out, (1, 4), (4096, 1)), out, t['x'][:1])
+    ref = R.linear(t['x'][:1], t['weight'], t['bias'], torch.ones(1, 4), 'relu')
+    R.check(out, ref['y'], ref['y_tol'], 'one row')
+    both = torch.zeros(6, 12, device=gpu_device)
+    both[:, :8] = t['x']
+    call(None, both[:, 8:], both[:, :8])
+    assert torch.equal(both[:, 8:], want - 1) and torch.equal(both[:, :8], t['x'])
+    with pytest.raises(ValueError, match='shares memory with x'):
+        call(None, both[:, 7:11], both[:, :8])

@@ -123,3 +123,33 @@ def test_linear_grid_limit():
         assert workspace((1 << 31) - 1, 8, 100, dtype, 0, 0) == 0
         assert workspace((1 << 31) - 1, 8, 100, dtype, 0, 1) == -4   # dx has 100
         assert workspace(1 << 30, 100, 8, dtype, 0, 0) == 0          # 2^23
+
+
+def test_results_apart_from_inputs():
+    """Shared memory is told by addresses alone: exactly, against the sets of elements."""
+    from tempo_amd import ops
+    buf = torch.zeros(64)
+    views = [torch.as_strided(buf, shape, stride, offset) for offset in (0, 1, 4, 6, 24)
+             for shape, stride in (((2, 3, 4), (12, 4, 1)), ((2, 3, 2), (12, 4, 1)),
+                                   ((2, 3, 2), (2, 4, 1)), ((3, 2, 2), (4, 12, 1)),
+                                   ((1, 1, 8), (5, 3, 1)), ((1, 3, 1), (7, 8, 9)))]
+
+    def elements(t):
+        return set(torch.arange(64).as_strided(t.shape, t.stride(), t.storage_offset())
+                   .flatten().tolist())
+
+    told = 0
+    for a in views:
+        for b in views:
+            shared = elements(a) & elements(b)
+            try:
+                ops._apart('out', a, x=b)
+                assert not shared
+                told += elements(b) & set(range(min(elements(a)), max(elements(a)))) != set()
+            except ValueError:
+                pass  # may be refused without need, too: only if their rows interleave
+            if max(elements(a)) < min(elements(b)) or max(elements(b)) < min(elements(a)):
+                ops._apart('out', a, x=b)
+    assert told > 20  # interleaved and apart: accepted
+    ops._apart('out', views[0][:0], x=views[0])
+    ops._apart('out', views[0], x=views[0][:0], weight=None)
