@@ -1326,6 +1326,15 @@ def _apart(name, out, **inputs):
                 raise ValueError(f'{name}: shares memory with {other}')
 
 
+def _rows_apart(name, t):
+    """No two rows of a result may share memory: each would be written by another thread."""
+    reach = t.shape[-1]
+    for apart, n in sorted((s, n) for n, s in zip(t.shape[:-1], t.stride()) if n > 1):
+        if apart < reach:
+            raise ValueError(f'{name}: its rows overlap')
+        reach += (n - 1) * apart
+
+
 def _like_time_order(t, channels):
     """Empty ``[B,T,channels]`` whose memory has time outermost where ``t``'s has."""
     B, T, _ = t.shape
@@ -1381,11 +1390,14 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
         _float_tensor(out, 'out', 3, gate.dtype, dev)
         if out.shape != gate.shape:
             raise ValueError(f'out: expected {tuple(gate.shape)}, got {tuple(out.shape)}')
-        _apart('out', out, gate=gate, value=value, state=state, state_out=state_out)
+        _rows_apart('out', out)
+        _apart('out', out, gate=gate, value=value, state=state, lengths=lengths,
+               state_out=state_out)
     last = _lane_state(state_out, 'state_out', B, D, dev)
     if last is not None:
         same = state is not None and state.data_ptr() == last.data_ptr()
-        _apart('state_out', last, gate=gate, value=value, state=None if same else state)
+        _apart('state_out', last, gate=gate, value=value, state=None if same else state,
+               lengths=lengths)
     else:
         last = gate.new_empty((B, D), dtype=torch.float32)
     if B == 0 or T == 0:

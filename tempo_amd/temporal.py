@@ -61,7 +61,7 @@ def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state
     fp32.  An infinity among the inputs leaves its channel's later states infinite or NaN.
 
     ``out`` / ``state_out`` (not under autograd): where to write the two results, apart from the
-    inputs in memory; only ``state_out`` may be ``state`` itself.
+    inputs in memory and no row over another; only ``state_out`` may be ``state`` itself.
 
     To capture a training step into a graph, drop eager results of the same leaves first: torch
     itself ends the process when a captured backward meets their gradient accumulators."""

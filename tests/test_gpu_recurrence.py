@@ -435,3 +435,39 @@ def test_strides_beyond_32_bits(gpu_device):
     want = tempo_amd.gated_recurrence(gate, value)
     got = tempo_amd.gated_recurrence(g, v)
     assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1])
+
+
+def test_result_rows_overlap(gpu_device):
+    """Rows of a result that coincide or run into each other are refused, as are results in the
+    memory of the lengths; rows of one batch item or one step alone may have any distance."""
+    import tempo_amd
+    gate, value = _inputs(3, 5, 6, torch.float32, gpu_device)
+    buf = torch.zeros(400, device=gpu_device)
+    lengths = torch.tensor([5, 2, 0], dtype=torch.int32, device=gpu_device)
+    want = tempo_amd.gated_recurrence(gate, value, lengths=lengths)
+
+    def call(strides, at=0, shape=(3, 5, 6), **kw):
+        out = torch.as_strided(buf, shape, strides, at)
+        h, last = tempo_amd.gated_recurrence(gate[:shape[0], :shape[1]],
+                                             value[:shape[0], :shape[1]], out=out,
+                                             lengths=lengths[:shape[0]], **kw)
+        assert h is out
+        return h, last
+
+    for strides in ((0, 6, 1), (30, 0, 1), (29, 6, 1), (30, 5, 1), (6, 17, 1), (0, 0, 1)):
+        with pytest.raises(ValueError, match='rows overlap'):
+            call(strides)
+    for strides in ((30, 6, 1), (6, 18, 1), (70, 13, 1), (7, 50, 1)):
+        got = call(strides)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    h, _ = call((0, 6, 1), shape=(1, 5, 6))
+    assert torch.equal(h, want[0][:1])
+    h, _ = call((6, 0, 1), shape=(3, 1, 6))
+    assert torch.equal(h[:2], want[0][:2, :1])
+    held = buf.view(torch.int32)[360:363]
+    held.copy_(lengths)
+    state = buf[358:376].view(3, 6)
+    with pytest.raises(ValueError, match='state_out: shares memory with lengths'):
+        tempo_amd.gated_recurrence(gate, value, lengths=held, state_out=state)
+    with pytest.raises(ValueError, match='out: shares memory with lengths'):
+        tempo_amd.gated_recurrence(gate, value, lengths=held, out=buf[300:390].view(3, 5, 6))

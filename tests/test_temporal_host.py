@@ -153,3 +153,14 @@ def test_results_apart_from_inputs():
     assert told > 20  # interleaved and apart: accepted
     ops._apart('out', views[0][:0], x=views[0])
     ops._apart('out', views[0], x=views[0][:0], weight=None)
+
+
+def test_rows_of_a_result_apart():
+    from tempo_amd import ops
+    buf = torch.zeros(400)
+    for shape, stride in (((3, 5, 6), (30, 6, 1)), ((3, 5, 6), (6, 18, 1)), ((1, 5, 6), (0, 6, 1)),
+                          ((3, 1, 6), (6, 0, 1)), ((0, 5, 6), (0, 6, 1)), ((4, 1), (1, 9))):
+        ops._rows_apart('out', torch.as_strided(buf, shape, stride))
+    for stride in ((0, 6, 1), (30, 0, 1), (29, 6, 1), (30, 5, 1), (6, 17, 1)):
+        with pytest.raises(ValueError):
+            ops._rows_apart('out', torch.as_strided(buf, (3, 5, 6), stride))
