@@ -1326,6 +1326,14 @@ def _apart(name, out, **inputs):
                 raise ValueError(f'{name}: shares memory with {other}')
 
 
+def _written(*results):
+    """Tells autograd that the caller's tensors hold new values: what was saved of them for a
+    backward pass, or computed from them, is out of date."""
+    given = [t for t in results if t is not None]
+    if given:
+        torch.autograd.graph.increment_version(given)
+
+
 def _rows_apart(name, t):
     """No two rows of a result may share memory: each would be written by another thread."""
     reach = t.shape[-1]
@@ -1380,7 +1388,8 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
     every ``RECURRENCE_SPAN``-th step, which :func:`recurrence_backward` starts from (None
     where ``T <= RECURRENCE_SPAN``: there ``state`` is all it needs)."""
     lib = _lib.load()
-    _no_grad_path('recurrence_forward', gate, value, state)
+    _no_grad_path('recurrence_forward', gate, value, state, out, state_out)
+    results = out, state_out
     gate, value, B, T, D = _recurrence_inputs(gate, value, lengths)
     dev = gate.device
     _lane_state(state, 'state', B, D, dev)
@@ -1413,6 +1422,7 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
     _launch('tempo_recurrence', dev, lib.tempo_recurrence, *_strided(gate), *_strided(value),
             _address(state), _address(lengths), *_strided(out), last.data_ptr(), _address(ckpt),
             B, T, D, code, _address(ws), need)
+    _written(*results)
     return out, last, ckpt
 
 
@@ -1521,12 +1531,12 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
     :func:`tempo_amd.fused_linear` with a 2-D weight.  ``pre``: the values before the activation
     as :func:`linear_backward` needs them (None unless ``want_pre`` and there is one)."""
     lib = _lib.load()
-    _no_grad_path('linear_forward', x, weight, bias, residual)
+    _no_grad_path('linear_forward', x, weight, bias, residual, out)
     act = _activation(activation)
     rows, M, N, K = _linear_operands(x, weight, bias)
     dev, code = x.device, FLOAT_DTYPES[x.dtype]
     shape = (*x.shape[:-1], N)
-    res, ldr = None, 0
+    res, ldr, result = None, 0, out
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or tuple(residual.shape) != shape:
             raise ValueError(f'residual: expected {list(shape)}, got '
@@ -1553,6 +1563,7 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
     _launch('tempo_linear', dev, lib.tempo_linear, rows.data_ptr(), rows.stride(0),
             weight.data_ptr(), weight.stride(0), _address(bias), _address(res), ldr,
             dst.data_ptr(), ldy, _address(pre), M, N, K, code, act, _address(ws), need)
+    _written(result)
     return out, pre
 
 

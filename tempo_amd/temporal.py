@@ -65,7 +65,7 @@ def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state
 
     To capture a training step into a graph, drop eager results of the same leaves first: torch
     itself ends the process when a captured backward meets their gradient accumulators."""
-    if _records(gate, value, state):
+    if _records(gate, value, state, out, state_out):
         if out is not None or state_out is not None:
             raise NotImplementedError('gated_recurrence: out / state_out are for calls without '
                                       'gradients (torch.no_grad() or detached tensors)')
@@ -112,7 +112,7 @@ def fused_linear(x, weight, bias=None, residual=None, activation='none', out=Non
     itself ends the process when a captured backward meets their gradient accumulators."""
     if isinstance(weight, torch.Tensor) and weight.dim() == 4 and weight.shape[2:] == (1, 1):
         weight = weight.flatten(1)
-    if _records(x, weight, bias, residual):
+    if _records(x, weight, bias, residual, out):
         if out is not None:
             raise NotImplementedError('fused_linear: out is for calls without gradients '
                                       '(torch.no_grad() or detached tensors)')

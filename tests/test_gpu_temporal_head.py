@@ -153,3 +153,57 @@ def test_parameters_and_refusals(gpu_device):
         head(maps, 5, T, state=torch.zeros(3, C, device=gpu_device))
     with pytest.raises(TypeError):
         head(maps.cpu(), 5, T)
+
+
+def test_results_in_place_are_seen_by_autograd(gpu_device):
+    """What was saved of a tensor, or computed from it, is out of date once it was out or
+    state_out: the backward pass says so, and the project layers unproject anew."""
+    import tempo_amd
+    x = torch.randn(6, 8, device=gpu_device)
+    w = torch.randn(8, 8, device=gpu_device)
+    leaf = torch.randn(6, 8, device=gpu_device, requires_grad=True)
+    gate, value = (torch.randn(3, 2, 8, device=gpu_device) for _ in range(2))
+
+    def linear(t):
+        tempo_amd.fused_linear(x, w, out=t)
+
+    def linear_over_residual(t):
+        tempo_amd.fused_linear(x, w, residual=t, out=t)
+
+    def states(t):
+        tempo_amd.gated_recurrence(gate, value, out=t.view(3, 2, 8))
+
+    def last_state(t):
+        tempo_amd.gated_recurrence(gate, value, state=t[:3], state_out=t[:3])
+
+    for write in (linear, linear_over_residual, states, last_state):
+        saved = torch.randn(6, 8, device=gpu_device)
+        loss = (leaf * saved).sum()
+        with torch.no_grad():
+            write(saved)
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()
+        with pytest.raises(NotImplementedError):
+            write(leaf)
+        with torch.inference_mode():
+            write(torch.zeros(6, 8, device=gpu_device))
+    before = x._version, w._version, gate._version
+    linear(torch.zeros(6, 8, device=gpu_device))
+    states(torch.zeros(6, 8, device=gpu_device))
+    assert before == (x._version, w._version, gate._version)
+
+    spec = dict(cfg='panoptic', B=1, cube=[12, 10, 9], hm='noise', joints=C, seed=901)
+    case = cases.to_device(cases.build_root(None, full=spec), gpu_device)
+    layer = tempo_amd.ProjectLayer(case['image_size'], case['heatmap_size'], 'mean')
+    maps = [m.contiguous(memory_format=torch.channels_last).requires_grad_(True)
+            for m in case['args'][0]]
+    old = layer.forward_zmax(maps, *case['args'][1:])
+    rows = maps[1].detach().permute(0, 2, 3, 1)
+    new = rows.clone()
+    with torch.no_grad():
+        tempo_amd.fused_linear(new, 2 * torch.eye(C, device=gpu_device),
+                               out=maps[1].permute(0, 2, 3, 1))
+    got = layer.forward_zmax(maps, *case['args'][1:])
+    fresh = tempo_amd.ProjectLayer(case['image_size'], case['heatmap_size'], 'mean')
+    assert torch.equal(got, fresh.forward_zmax(maps, *case['args'][1:]))
+    assert not torch.equal(got, old)
