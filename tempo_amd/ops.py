@@ -8,6 +8,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, numerics
 
@@ -68,10 +69,20 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
 
 
+def _no_tangent(what, *tensors):
+    """No kernel carries forward-mode derivatives (which ``no_grad`` does not turn off): a result
+    without a tangent would count as a constant."""
+    if forward_ad._current_level >= 0 and any(
+            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
+            for t in tensors):
+        raise NotImplementedError(f'{what} has no forward-mode derivative')
+
+
 def _no_grad_path(what, *tensors):
     """Forward-only entry points raise when autograd would expect a gradient through them
     (the torch expressions they replace carry one); silently cutting the graph would train
     on wrong gradients."""
+    _no_tangent(what, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(
             f'{what} is forward-only: call it under torch.no_grad() / on detached tensors, '
@@ -1450,6 +1461,7 @@ def recurrence_backward(grad_h, grad_last, gate, value=None, state=None, ckpt=No
 
 def _recurrence_backward(grad_h, grad_last, gate, value, state, ckpt, lengths, want_state):
     """The same on arguments that are known to fit (``grad_h``: channels adjacent)."""
+    _no_tangent('recurrence_backward', grad_h, grad_last, gate, value, state)
     both = value is None
     B, T, D = gate.shape
     dgate = _like_time_order(gate, D)
@@ -1584,6 +1596,7 @@ def linear_backward(grad_y, x, weight, pre=None, activation='none', want=(True, 
 
 def _linear_backward(grad_y, x, weight, pre, act, want):
     """The same on arguments that are known to fit (``grad_y``: any strides)."""
+    _no_tangent('linear_backward', grad_y, x, weight)
     N, K = weight.shape
     M = x.numel() // K
     dx = x.new_empty(x.shape) if want[0] else None

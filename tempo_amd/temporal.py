@@ -5,7 +5,8 @@ used at ``tempo/models/model_utils.py:10-16``), one step after the other.  Here 
 on the input alone, so that the recurrence is linear and runs over a whole sequence in one pass.
 
 Everything runs in HIP kernels on the current stream; there is no CPU path.  The backward
-passes use no atomics: gradients do not change from run to run.
+passes use no atomics: gradients do not change from run to run.  There are no forward-mode
+derivatives; asking for one raises.
 """
 import torch
 from torch.autograd.function import once_differentiable

@@ -207,3 +207,54 @@ def test_results_in_place_are_seen_by_autograd(gpu_device):
     fresh = tempo_amd.ProjectLayer(case['image_size'], case['heatmap_size'], 'mean')
     assert torch.equal(got, fresh.forward_zmax(maps, *case['args'][1:]))
     assert not torch.equal(got, old)
+
+
+@pytest.mark.parametrize('grad_mode', [True, False])
+def test_forward_mode_is_refused(grad_mode, gpu_device):
+    """A tangent of any tensor that the results depend on: the call raises, it returns no
+    constant.  Tensors without one pass inside of a dual level."""
+    import torch.autograd.forward_ad as fwd
+
+    import tempo_amd
+    from tempo_amd import ops
+    gen = torch.Generator(device=gpu_device).manual_seed(0)
+
+    def some(*shape):
+        return torch.randn(*shape, generator=gen, device=gpu_device)
+
+    def dual(t):
+        return fwd.make_dual(t, torch.ones_like(t))
+
+    linear = [some(5, 8), some(4, 8), some(4), some(5, 4)]
+    rec = [some(2, 3, 8), some(2, 3, 8), some(2, 8)]
+    leaf, leaf3 = linear[0].clone().requires_grad_(True), rec[0].clone().requires_grad_(True)
+    y, (h, last) = tempo_amd.fused_linear(leaf, linear[1]), tempo_amd.gated_recurrence(leaf3, rec[1])
+    with torch.set_grad_enabled(grad_mode), fwd.dual_level():
+        for i in range(4):
+            args = [dual(t) if i == j else t for j, t in enumerate(linear)]
+            with pytest.raises(NotImplementedError):
+                tempo_amd.fused_linear(*args, activation='gelu')
+            with pytest.raises(NotImplementedError):
+                tempo_amd.fused_linear(*[a if i == j else a.clone().requires_grad_(True)
+                                         for j, a in enumerate(args)])
+            with pytest.raises(NotImplementedError):
+                ops.linear_forward(*args)
+        for i in range(3):
+            args = [dual(t) if i == j else t for j, t in enumerate(rec)]
+            with pytest.raises(NotImplementedError):
+                tempo_amd.gated_recurrence(*args)
+            with pytest.raises(NotImplementedError):
+                ops.recurrence_forward(*args)
+        assert torch.equal(tempo_amd.fused_linear(linear[0], linear[1]), y)
+        assert torch.equal(tempo_amd.gated_recurrence(*rec[:2])[1], last)
+        for call in (lambda: torch.autograd.grad(y, leaf, dual(torch.ones_like(y)),
+                                                 retain_graph=True),
+                     lambda: torch.autograd.grad(h, leaf3, dual(torch.ones_like(h)),
+                                                 retain_graph=True),
+                     lambda: torch.autograd.grad(last, leaf3, dual(torch.ones_like(last)),
+                                                 retain_graph=True)):
+            with pytest.raises(NotImplementedError):
+                call()
+    with pytest.raises(RuntimeError):  # function transforms hand over tensors without memory
+        torch.func.jvp(lambda x: tempo_amd.fused_linear(x, linear[1]), (linear[0],),
+                       (torch.ones_like(linear[0]),))
