@@ -25,7 +25,7 @@ FLAGS = ['--offload-arch=gfx950', '-O3', '-fPIC', '-std=c++17', '-Wall',
 SOURCES = {
     'tempo_unproject.hip': (['unproject_math.h'], ['-ffp-contract=off']),
     'recurrence.hip': ([], []),
-    'linear.hip': ([], []),
+    'linear.hip': (['linear_plan.h'], []),
 }
 
 

@@ -490,3 +490,26 @@ def test_out_and_residual_overlap(gpu_device):
     assert torch.equal(both[:, 8:], bare) and torch.equal(both[:, :8], t['x'])
     with pytest.raises(ValueError, match='shares memory with x'):
         call(None, both[:, 7:11], both[:, :8])
+
+
+# (M, K, N) with, in 16 bits, one product in 256 x 256 tiles: the forward, dx or dW, with
+# remainders of rows, columns and k, sums shorter than the stages in flight, more tiles than
+# compute units.  Which kernel a size selects is asserted without a GPU, in test_linear_plan.py.
+WIDEST = [(4000, 520, 4008, 'y'), (4040, 1032, 4008, 'y'), (6000, 72, 4104, 'y'),
+          (5000, 264, 6152, 'y'), (4040, 4008, 1032, 'dx'), (1032, 4008, 4040, 'dweight')]
+# fp32 products in tiles of 64 x 128 that no size above selects
+NARROW = [(9, 17209, 8), (8, 17472, 8), (13, 18688, 8), (184, 8, 8208), (47, 8, 16599)]
+
+
+@pytest.mark.parametrize('dtype', DTYPES[1:], ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', WIDEST, ids=str)
+def test_widest_tiles(shape, dtype, gpu_device):
+    M, K, N, _ = shape
+    _check_grads(_make(M, K, N, dtype, gpu_device, seed=40, residual=True, grad=True), 'gelu')
+
+
+@pytest.mark.parametrize('shape', NARROW, ids=str)
+def test_narrow_tiles(shape, gpu_device):
+    M, K, N = shape
+    _check_grads(_make(M, K, N, torch.float32, gpu_device, seed=41, residual=True, grad=True),
+                 'silu')
