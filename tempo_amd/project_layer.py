@@ -97,7 +97,8 @@ class RecurrentProcessLayerNHWC(nn.Module):
     ``T*V*B`` images as ``rnn_multiview_pose.py:321`` stacks them (a ``torch.channels_last`` map
     is read where it lies, another one is copied into that order) and returns
     ``(feature_maps, state)``: ``feature_maps[t][v]`` is ``[B,C,H,W]`` in channels_last memory,
-    which the project layers read in place, and ``state`` (fp32 ``[V*B*H*W, C]``) goes into the
+    which the project layers read in place if it is fp32 (16-bit maps they copy to NCHW order and
+    widen, as those of any other head), and ``state`` (fp32 ``[V*B*H*W, C]``) goes into the
     next call, so that a recording can be fed one timestep at a time.  Trains through both
     operators (:mod:`tempo_amd.temporal`); half-precision maps run in their own type."""
 

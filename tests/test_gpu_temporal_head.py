@@ -258,3 +258,41 @@ def test_forward_mode_is_refused(grad_mode, gpu_device):
     with pytest.raises(RuntimeError):  # function transforms hand over tensors without memory
         torch.func.jvp(lambda x: tempo_amd.fused_linear(x, linear[1]), (linear[0],),
                        (torch.ones_like(linear[0]),))
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16], ids=lambda d: str(d)[6:])
+def test_half_precision_head_and_unprojection_together(dtype, gpu_device):
+    """16-bit maps are widened exactly on their way into the volume: the same values as fp32
+    copies of them, in any memory order, and the same gradients up to one rounding of each."""
+    import tempo_amd
+    spec = dict(cfg='panoptic', B=2, cube=[12, 10, 9], hm='noise', joints=C, seed=902)
+    case = cases.to_device(cases.build_root(None, full=spec), gpu_device)
+    V = len(case['args'][0])
+    hw = tuple(case['args'][0][0].shape[2:])
+    head, maps = _head(gpu_device, dtype, hw=hw, V=V)
+    layer = tempo_amd.ProjectLayer(case['image_size'], case['heatmap_size'], 'mean')
+    rest = case['args'][1:]
+    out, _ = head(maps, V, T)
+    assert all(m.dtype == dtype for ms in out for m in ms)
+    with torch.no_grad():
+        for ms in out:
+            volume = layer(ms, *rest)[0]
+            assert volume.dtype == torch.float32
+            for other in ([m.contiguous() for m in ms], [m.float() for m in ms],
+                          [m.float().contiguous() for m in ms]):
+                assert torch.equal(layer(other, *rest)[0], volume)
+    volume = layer(out[1], *rest)[0]
+    seed = torch.randn(volume.shape, device=gpu_device,
+                       generator=torch.Generator(device=gpu_device).manual_seed(3))
+    wide = [m.detach().float().requires_grad_(True) for m in out[1]]
+    want = torch.autograd.grad(layer(wide, *rest)[0], wide, seed)
+    size = torch.autograd.grad(layer(wide, *rest)[0], wide, seed.abs())
+    got = torch.autograd.grad(volume, out[1], seed, retain_graph=True)
+    for a, b, c in zip(got, want, size):
+        assert a.dtype == dtype
+        # the unprojection's atomics add at most 1080 terms in another order
+        lim = R.rounding(b.double(), dtype) + 1.01 * 1080 * 2.0 ** -24 * c.double().abs()
+        assert bool(((a.double() - b.double()).abs() <= lim).all())
+    grads = torch.autograd.grad(volume, [head.weight, head.bias], seed)
+    for g, p in zip(grads, (head.weight, head.bias)):
+        assert g.dtype == p.dtype and bool(torch.isfinite(g).all()) and bool(g.any())
