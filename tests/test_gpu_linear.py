@@ -513,3 +513,24 @@ def test_narrow_tiles(shape, gpu_device):
     M, K, N = shape
     _check_grads(_make(M, K, N, torch.float32, gpu_device, seed=41, residual=True, grad=True),
                  'silu')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+def test_gelu_far_down_its_tail(dtype, gpu_device):
+    """K = 1 and a weight of 1, so that z is exact: gelu and its slope to one rounding and 2^-16 of
+    their terms.  16 bits: 2^-18 of the approximation and 2^-24 z^2 / 2 for each rounding of the
+    exponential's argument, three of them make 2^-17 at z = -9.  fp32: erfc(x) changes by
+    2 x^2 + 1 = z^2 + 1 <= 82 times its argument's relative error, which is 2^-24 of the product
+    and 2^-25.8 of the constant 1 / sqrt 2, 2^-17.3 in all, and the library's erfc errs itself."""
+    z = torch.cat([torch.linspace(-9, 9, 3001), -torch.logspace(-4, 0.9, 500)]).to(dtype)
+    z = z[:, None].to(gpu_device)
+    one = torch.ones(1, 1, dtype=dtype, device=gpu_device)
+    t = {'x': z, 'weight': one, 'bias': None, 'residual': None, 'grad': torch.ones_like(z)}
+    y, g = _train(t, 'gelu')
+    z = z.double().cpu()
+    phi = torch.erfc(-z * 0.5 ** 0.5) / 2  # special.ndtr is (1 + erf) / 2: it cancels
+    bell = torch.exp(-z * z / 2) * 0.3989422804014327
+    own = 2.0 ** -16
+    R.check(y, z * phi, R.rounding(z * phi, dtype) + own * (z * phi).abs(), 'gelu')
+    R.check(g['x'], phi + z * bell, R.rounding(phi + z * bell, dtype) +
+            own * (phi + z.abs() * bell), 'slope')
