@@ -72,10 +72,9 @@ def _ptr(t):
 def _no_tangent(what, *tensors):
     """No kernel carries forward-mode derivatives (which ``no_grad`` does not turn off): a result
     without a tangent would count as a constant."""
-    if forward_ad._current_level >= 0 and any(
-            isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None
-            for t in tensors):
-        raise NotImplementedError(f'{what} has no forward-mode derivative')
+    for t in tensors if forward_ad._current_level >= 0 else ():
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'{what} has no forward-mode derivative')
 
 
 def _no_grad_path(what, *tensors):
@@ -1340,9 +1339,9 @@ def _apart(name, out, **inputs):
 def _written(*results):
     """Tells autograd that the caller's tensors hold new values: what was saved of them for a
     backward pass, or computed from them, is out of date."""
-    given = [t for t in results if t is not None]
-    if given:
-        torch.autograd.graph.increment_version(given)
+    for t in results:
+        if t is not None:
+            torch.autograd.graph.increment_version(t)
 
 
 def _rows_apart(name, t):
