@@ -108,16 +108,22 @@ class RecurrentProcessLayerNHWC(nn.Module):
         self.weight, self.bias = conv.weight, conv.bias
 
     def forward(self, backbone_map, num_views, timesteps=1, state=None):
+        if not isinstance(backbone_map, torch.Tensor) or backbone_map.dim() != 4:
+            raise ValueError('backbone_map must be [timesteps * num_views * batch, K, H, W]')
         images, K, H, W = backbone_map.shape
         T, V = int(timesteps), int(num_views)
+        if T < 1 or V < 1:
+            raise ValueError(f'timesteps and num_views must be positive, got {T} and {V}')
         if images % (T * V):
             raise ValueError('backbone_map.shape[0] must be timesteps * num_views * batch')
+        if K != self.weight.shape[1]:
+            raise ValueError(f'backbone_map has {K} channels, the layer {self.weight.shape[1]}')
         B, C = images // (T * V), int(self.weight.shape[0]) // 2
         rows = backbone_map.contiguous(memory_format=torch.channels_last).permute(0, 2, 3, 1)
         both = fused_linear(rows.reshape(-1, K), self.weight.to(backbone_map.dtype),
                             self.bias.to(backbone_map.dtype))
         # one lane per view, batch item, texel and channel; time outermost in memory
-        h, state = gated_recurrence(both.view(T, -1, 2 * C).transpose(0, 1), state=state)
+        h, state = gated_recurrence(both.view(T, V * B * H * W, 2 * C).transpose(0, 1), state=state)
         maps = h.transpose(0, 1).view(T, V, B, H, W, C).permute(0, 1, 2, 5, 3, 4)
         return [[maps[t, v] for v in range(V)] for t in range(T)], state
 

@@ -296,3 +296,22 @@ def test_half_precision_head_and_unprojection_together(dtype, gpu_device):
     grads = torch.autograd.grad(volume, [head.weight, head.bias], seed)
     for g, p in zip(grads, (head.weight, head.bias)):
         assert g.dtype == p.dtype and bool(torch.isfinite(g).all()) and bool(g.any())
+
+
+def test_recurrent_process_layer_on_nothing_and_on_one_texel(gpu_device):
+    """No images, maps without texels: empty results of the right shapes; maps of a single texel
+    are channel-last in any order."""
+    head, maps = _head(gpu_device)
+    for images, hw, T_ in ((0, (4, 6), 2), (10, (0, 6), 2), (10, (4, 0), 1)):
+        out, state = head(torch.zeros(images, K, *hw, device=gpu_device), 5, T_)
+        B = images // (5 * T_)
+        assert len(out) == T_ and all(m.shape == (B, C) + hw for ms in out for m in ms)
+        assert state.shape == (5 * B * hw[0] * hw[1], C)
+    with torch.no_grad():
+        one = maps[:, :, 3:4, 7:8]
+        for m in (one, one.contiguous(), one.contiguous(memory_format=torch.channels_last)):
+            out, state = head(m, 5, T)
+            _, rec, _, moved = _reference(head, m, 5)
+            got = torch.stack([torch.stack(ms) for ms in out]).permute(1, 2, 4, 5, 0, 3)
+            R.check(got.reshape(-1, T, C), rec['h'], rec['h_tol'] + moved, 'maps')
+            R.check(state, rec['last'], rec['last_tol'] + moved[:, 0], 'state')

@@ -164,3 +164,15 @@ def test_rows_of_a_result_apart():
     for stride in ((0, 6, 1), (30, 0, 1), (29, 6, 1), (30, 5, 1), (6, 17, 1)):
         with pytest.raises(ValueError):
             ops._rows_apart('out', torch.as_strided(buf, (3, 5, 6), stride))
+
+
+def test_recurrent_process_layer_refusals():
+    """Before any kernel: counts that divide nothing, other ranks and channels."""
+    import tempo_amd
+    head = tempo_amd.RecurrentProcessLayerNHWC(8, 4)
+    maps = torch.zeros(6, 8, 3, 5)
+    for bad in (lambda: head(maps, 0), lambda: head(maps, 3, 0), lambda: head(maps, -3, -2),
+                lambda: head(maps, -6), lambda: head(maps, 4), lambda: head(maps, 3, 4),
+                lambda: head(maps[0], 1), lambda: head(maps[:, :7], 3, 2), lambda: head(None, 1)):
+        with pytest.raises(ValueError):
+            bad()
