@@ -534,3 +534,37 @@ def test_gelu_far_down_its_tail(dtype, gpu_device):
     R.check(y, z * phi, R.rounding(z * phi, dtype) + own * (z * phi).abs(), 'gelu')
     R.check(g['x'], phi + z * bell, R.rounding(phi + z * bell, dtype) +
             own * (phi + z.abs() * bell), 'slope')
+
+
+# long sums, in one piece and split: rows, k, columns (fp32 kernels of every kind)
+EXACT = [(4, 4095, 24), (64, 4096, 512), (130, 4096, 136), (131, 4093, 77), (33000, 511, 24),
+         (33000, 512, 32), (1024, 4096, 1024), (513, 1021, 515)]
+
+
+@pytest.mark.parametrize('shape', EXACT, ids=str)
+def test_long_fp32_sums_lose_nothing(shape, gpu_device):
+    """Whole numbers whose sums stay below 2^24: every order of fp32 additions is exact, so the
+    forward pass and all gradients are, to the last bit.  One factor takes 9 to 12 bits (the other
+    one is -1, 0 or 1), more than bf16 or, where it is 12, fp16 operands hold: none may be
+    shortened on its way, which bounds for rounded sums of this length would not show."""
+    M, K, N = shape
+    gen = torch.Generator().manual_seed(M)
+
+    def wide(rows, cols, terms):  # |sum of `terms` of them| < 2^24
+        most = min(4095, (2 ** 24 - 1) // terms)
+        assert most > 2 ** 8
+        return torch.randint(-most, most + 1, (rows, cols), generator=gen).float()
+
+    def signs(rows, cols):
+        return torch.randint(-1, 2, (rows, cols), generator=gen).float()
+
+    for x, w, g in ((wide(M, K, max(K, M)), signs(N, K), signs(M, N)),
+                    (signs(M, K), wide(N, K, max(K, N)), signs(M, N)),
+                    (signs(M, K), signs(N, K), wide(M, N, max(M, N)))):
+        t = {'x': x, 'weight': w, 'bias': None, 'residual': None, 'grad': g}
+        t = {k: v if v is None else v.to(gpu_device) for k, v in t.items()}
+        y, got = _train(t, 'none')
+        x, w, g = x.double(), w.double(), g.double()
+        assert torch.equal(y.double().cpu(), x @ w.t())
+        assert torch.equal(got['x'].double().cpu(), g @ w)
+        assert torch.equal(got['weight'].double().cpu(), g.t() @ x)
