@@ -105,7 +105,8 @@ def fused_linear(x, weight, bias=None, residual=None, activation='none', out=Non
 
     Sums are fp32, the result is rounded once; fp32 inputs are multiplied in fp32.
     Differentiable once, with respect to every tensor; for the backward pass the value in front
-    of the activation is kept in x's type, as a layer's output would be.  ``out`` (not under
+    of the activation is kept in x's type, as a layer's output would be.  relu's slope is that of
+    the sum as computed: 0 or 1 where the sum lies within its rounding of 0.  ``out`` (not under
     autograd): where to write the result; it may be the residual (the same memory in the same
     order), but share none with the other inputs.
 

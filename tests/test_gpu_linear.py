@@ -568,3 +568,32 @@ def test_long_fp32_sums_lose_nothing(shape, gpu_device):
         assert torch.equal(y.double().cpu(), x @ w.t())
         assert torch.equal(got['x'].double().cpu(), g @ w)
         assert torch.equal(got['weight'].double().cpu(), g.t() @ x)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('shape', [(153600, 256, 32), (4999, 251, 515), (5000, 256, 520),
+                                   (700, 64, 40), (12, 256, 64)], ids=str)
+def test_relu_of_exact_sums(shape, dtype, gpu_device):
+    """relu's slope is discontinuous: where z lies within rounding of 0, two right programs may
+    differ by a whole gradient.  On operands with few bits every sum is exact in any order, z's
+    signs are, and the training step has to be: y, dx, dW and db are the 64-bit values, rounded
+    once.  (x: multiples of 2^-6 up to 1, weight: of 2^-9 up to 55 of them, so that
+    |z| 2^15 <= 64 x 55 x 256 < 2^24, and dW 2^6 <= 64 M < 2^24.)"""
+    M, K, N = shape
+    gen = torch.Generator().manual_seed(M)
+
+    def lattice(most, step, *size):
+        return torch.randint(-most, most + 1, size, generator=gen).float() * step
+
+    t = {'x': lattice(64, 2.0 ** -6, M, K), 'weight': lattice(55, 2.0 ** -9, N, K),
+         'bias': lattice(100, 2.0 ** -15, N), 'grad': lattice(1, 1.0, M, N)}
+    x, w, b, g = (t[k].double() for k in ('x', 'weight', 'bias', 'grad'))
+    z = x @ w.t() + b
+    dz = g * (z > 0)
+    want = {'x': dz @ w, 'weight': dz.t() @ x, 'bias': dz.sum(0)}
+    t = {k: v.to(dtype).to(gpu_device) for k, v in t.items()}
+    assert all(torch.equal(t[k].cpu().double(), v) for k, v in zip(t, (x, w, b, g)))
+    y, got = _train(dict(t, residual=None), 'relu')
+    assert torch.equal(y.cpu(), z.clamp(min=0).to(dtype))
+    for k in want:
+        assert torch.equal(got[k].cpu(), want[k].to(dtype)), k
