@@ -169,11 +169,11 @@ template <typename T>
 struct Gate {
   float z, f;
   __device__ __forceinline__ explicit Gate(float g) {
-    float a = -1.44269504088896341f * g;
-    a = a > 126.f ? 126.f : a;  // f below: no infinity times 0; a NaN passes
+    float a = 1.44269504088896341f * g;
+    a = a > 126.f ? 126.f : a;  // z below: no infinity times 0; a NaN passes
     const float e = __builtin_amdgcn_exp2f(a);
-    z = __builtin_amdgcn_rcpf(1.f + e);
-    f = e * z;
+    f = __builtin_amdgcn_rcpf(1.f + e);
+    z = e * f;  // 0 where the gate is shut for good: the value may be the type's largest there
   }
   __device__ __forceinline__ float step(float h, float v) const { return fmaf(z, v - h, h); }
   __device__ __forceinline__ float back(float x) const { return f * x; }

@@ -471,3 +471,35 @@ def test_result_rows_overlap(gpu_device):
         tempo_amd.gated_recurrence(gate, value, lengths=held, state_out=state)
     with pytest.raises(ValueError, match='out: shares memory with lengths'):
         tempo_amd.gated_recurrence(gate, value, lengths=held, out=buf[300:390].view(3, 5, 6))
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=lambda d: str(d)[6:])
+@pytest.mark.parametrize('T', [1, 3, 2000])
+def test_shut_gates_hide_the_largest_values(T, dtype, gpu_device):
+    """Steps masked by their gate (minus infinity, the type's lowest value, -110) may hold the
+    type's lowest or largest value, too: the state stays, bit for bit, and no gradient comes out
+    of them."""
+    gate, value = _inputs(2, T, 9, dtype, gpu_device, seed=70)
+    state, grad_last = _states(2, 9, gpu_device)
+    info = torch.finfo(dtype)
+    for low in (float('-inf'), info.min, -110.0):
+        gate.fill_(low)
+        for most in (info.min, info.max):
+            value.fill_(most)
+            h, last, g = _train(gpu_device, gate, value, state, None, torch.zeros_like(gate),
+                                grad_last)
+            assert torch.equal(last, state)
+            assert torch.equal(h, state.to(dtype)[:, None].expand_as(h))
+            assert torch.equal(g['state'], grad_last)
+            if low != -110.0:
+                assert not bool(g['gate'].any()) and not bool(g['value'].any())
+    # among ordinary steps
+    gate, value = _inputs(2, T, 9, dtype, gpu_device, seed=71)
+    masked = torch.arange(T, device=gpu_device) % 3 == 1
+    gate[:, masked] = float('-inf')
+    value[:, masked] = 0
+    ref = R.recurrence(gate, value, state)
+    value[:, masked] = info.min
+    h, last, _ = _train(gpu_device, gate, value, state, None, torch.zeros_like(gate), grad_last)
+    R.check(h, ref['h'], ref['h_tol'], 'h')
+    R.check(last, ref['last'], ref['last_tol'], 'last')
