@@ -15,7 +15,8 @@
 // shortened operands).  The epilogue is fp32 and rounds y once.  Two choices round to the
 // tensors' type in between: z is kept for the backward pass in that type, and dz is an operand
 // of two products in that type; both are half a step of a value that the products average
-// over, no more than the rounding of their outputs.  db is summed from unrounded dz.
+// over, no more than the rounding of their outputs (in fp16 a dz below 2^-25 becomes 0, like any
+// gradient of that type: losses are scaled).  db is summed from unrounded dz.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -641,7 +642,7 @@ __global__ __launch_bounds__(kThreads) void tile_kernel(const TileArgs a) {
 // product reads from LDS.  16384 x 4096 x 4096 in bf16: 464 us bare (1.18 PFLOP/s; the library's
 // product 354 us), 523 us with a residual; what bounds it is the way from L2 to LDS -- on loads
 // that all miss memory the same loop runs at 2.1 PFLOP/s, on loads that hit L2 at 1.42 -- and at
-// short k the epilogue, which nothing overlaps (8192 x 4096 x 1024: 75 us bare, 117 with gelu and
+// short k the epilogue, which nothing overlaps (8192 x 4096 x 1024: 75 us bare, 119 with gelu and
 // the values kept for the backward pass).  128 x 256 tiles, two workgroups a compute unit, do
 // overlap it and lose more in the loop (600 us).  Chunks outside an operand carry an offset beyond the buffer's
 // range, for which the hardware writes zeros.  A chunk's place in LDS follows from its lane
@@ -1147,7 +1148,7 @@ __device__ __forceinline__ void slopes(const Chunk& z, float (&d)[V], int act) {
 // dz = g * act'(z) in the tensors' type (unless dz is NULL) and the sums of the unrounded
 // values over the workgroup's rows (right into db where one workgroup holds them all).  A thread
 // owns 16 bytes of columns, WIDE threads side by side, four rows of each under way at a time: 8192
-// x 4096 in bf16 39 us, 5.2 TB/s.
+// x 4096 in bf16 42 us, 4.8 TB/s.
 template <typename T, int WIDE>
 __global__ __launch_bounds__(kThreads) void grad_z_kernel(const T* g, long long ldg, const T* pre,
                                                           T* dz, float* sums, T* db, long long M,

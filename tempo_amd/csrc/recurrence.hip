@@ -26,10 +26,12 @@
 // chunk's A is kept as S = 1 - A while S < 1/2 for the same reason (encoded as +S, otherwise
 // as -A).
 //
+// Values and states are taken from each other: a difference beyond fp32's range overflows.
+//
 // Measured (rates of a large copy on the same card: 4.8 TB/s, of a large sum 4.0 TB/s): where
-// lanes fill the card, one pass each, 153600 x 4 x 32 in fp32 forward 50 us (4.7 TB/s),
-// backward 74 us (5.3 TB/s).  Cut in time, the inputs are read twice: 1 x 65536 x 1024 in bf16
-// 73 + 13 + 76 us (3.7 and 5.3 TB/s of what the two passes move).  One pass would need
+// lanes fill the card, one pass each, 153600 x 4 x 32 in fp32 forward 54 us (4.8 TB/s),
+// backward 73 us (5.4 TB/s).  Cut in time, the inputs are read twice: 1 x 65536 x 1024 in bf16
+// 77 + 14 + 75 us (3.6 and 5.4 TB/s of what the two passes move).  One pass would need
 // workgroups that wait for each other; re-reading is what it costs not to.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -537,8 +539,10 @@ struct Plan {
 
 // Threads hold 4 channels; the backward beyond 4 steps 2, for its registers hold a span of
 // fp32 values (8 x 2048 x 1024 in bf16: 34 us against 42 with 4, 256 registers).  Time is cut
-// only where the (b, d) lanes alone are fewer than kFill threads, 16 waves for each of the
-// 256 compute units' 4 SIMDs (1 x 65536 x 1024: 68 us for the last pass, 80 with half of that).
+// only where the (b, d) lanes alone are fewer than kFill threads: 16 waves for each of the 256
+// compute units, 4 for each of their SIMDs.  Sums of the kernels' times with a quarter of that,
+// half, as it is and twice, in us: 8 x 2048 x 1024 in bf16 trained 140, 112, 109, 110; forward of
+// 1 x 65536 x 1024 187, 154, 164, 162.
 constexpr uint32_t kFill = 1u << 18;
 constexpr uint32_t kMinChunk = 2 * kSpan;
 

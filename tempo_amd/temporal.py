@@ -59,7 +59,8 @@ def gated_recurrence(gate, value=None, state=None, lengths=None, out=None, state
     Returns ``(h [B,T,D], last [B,D])``: every state in the inputs' type and the fp32 state
     after the last step, to go on from (a serving loop passes T = 1 and the carried state).
     Differentiable once, with respect to ``gate``, ``value`` and ``state``.  States and sums are
-    fp32.  An infinity among the inputs leaves its channel's later states infinite or NaN.
+    fp32.  An infinity among the inputs leaves its channel's later states infinite or NaN, as does
+    a value whose difference from the state in front of it is beyond fp32's range.
 
     ``out`` / ``state_out`` (not under autograd): where to write the two results, apart from the
     inputs in memory and no row over another; only ``state_out`` may be ``state`` itself.
