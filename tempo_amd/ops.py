@@ -82,7 +82,8 @@ def _no_grad_path(what, *tensors):
     (the torch expressions they replace carry one); silently cutting the graph would train
     on wrong gradients."""
     _no_tangent(what, *tensors)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                       for t in tensors):
         raise NotImplementedError(
             f'{what} is forward-only: call it under torch.no_grad() / on detached tensors, '
             'or use the torch expression it replaces for a training step')
@@ -1403,6 +1404,7 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
     gate, value, B, T, D = _recurrence_inputs(gate, value, lengths)
     dev = gate.device
     _lane_state(state, 'state', B, D, dev)
+    last = _lane_state(state_out, 'state_out', B, D, dev)
     if out is None:
         out = _like_time_order(gate, D)
     else:
@@ -1411,8 +1413,7 @@ def recurrence_forward(gate, value=None, state=None, lengths=None, out=None, sta
             raise ValueError(f'out: expected {tuple(gate.shape)}, got {tuple(out.shape)}')
         _rows_apart('out', out)
         _apart('out', out, gate=gate, value=value, state=state, lengths=lengths,
-               state_out=state_out)
-    last = _lane_state(state_out, 'state_out', B, D, dev)
+               state_out=last)
     if last is not None:
         same = state is not None and state.data_ptr() == last.data_ptr()
         _apart('state_out', last, gate=gate, value=value, state=None if same else state,
@@ -1558,8 +1559,8 @@ def linear_forward(x, weight, bias=None, residual=None, activation='none', out=N
         out = dst = x.new_empty(shape)
         ldy = N
     else:
-        if tuple(out.shape) != shape:
-            raise ValueError(f'out: expected {list(shape)}, got {list(out.shape)}')
+        if not isinstance(out, torch.Tensor) or tuple(out.shape) != shape:
+            raise ValueError(f'out: expected {list(shape)}, got {list(getattr(out, "shape", []))}')
         dst = _rows(out, 'out', x.dtype, dev)
         ldy = dst.stride(0)
         if M > 1 and ldy < N:

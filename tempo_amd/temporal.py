@@ -15,7 +15,8 @@ from . import ops
 
 
 def _records(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad
+                                           for t in tensors)
 
 
 class _GatedRecurrence(torch.autograd.Function):

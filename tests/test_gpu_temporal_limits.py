@@ -207,3 +207,21 @@ def test_smallest_numbers_count(dtype, gpu_device):
     gate = torch.full((3, 1, 1), float('inf'), dtype=dtype, device=gpu_device)
     h, last = tempo_amd.gated_recurrence(gate, x[:, None])
     assert torch.equal(h, x[:, None]) and torch.equal(last.double().cpu(), tiny)
+
+
+def test_arguments_that_are_no_tensors(gpu_device):
+    import tempo_amd
+    x, w = torch.zeros(2, 8, device=gpu_device), torch.zeros(4, 8, device=gpu_device)
+    gate, state = torch.zeros(2, 3, 8, device=gpu_device), torch.zeros(2, 8, device=gpu_device)
+    for bad in (lambda: tempo_amd.fused_linear(x, 3.0), lambda: tempo_amd.fused_linear(x, w, 1.0),
+                lambda: tempo_amd.fused_linear(x, w, residual=1.0),
+                lambda: tempo_amd.fused_linear(x, w, out=[1.0]),
+                lambda: tempo_amd.fused_linear(x, w, activation=None),
+                lambda: tempo_amd.gated_recurrence(gate, 1.0),
+                lambda: tempo_amd.gated_recurrence(gate, gate, state=0.0),
+                lambda: tempo_amd.gated_recurrence(gate, gate, state, lengths=[3, 3]),
+                lambda: tempo_amd.gated_recurrence(gate, gate, state, out=[1.0]),
+                lambda: tempo_amd.gated_recurrence(gate, gate, state, out=gate.clone(),
+                                                   state_out=1.0)):
+        with pytest.raises((TypeError, ValueError)):
+            bad()

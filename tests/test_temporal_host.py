@@ -176,3 +176,16 @@ def test_recurrent_process_layer_refusals():
                 lambda: head(maps[0], 1), lambda: head(maps[:, :7], 3, 2), lambda: head(None, 1)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_arguments_that_are_no_tensors():
+    import tempo_amd
+    x = torch.zeros(2, 3, 8)
+    for bad in (lambda: tempo_amd.fused_linear([1.0, 2.0], x[0]),
+                lambda: tempo_amd.fused_linear(x.numpy(), x[0]),
+                lambda: tempo_amd.fused_linear(None, None),
+                lambda: tempo_amd.gated_recurrence([1.0, 2.0], x),
+                lambda: tempo_amd.gated_recurrence(x.numpy(), x.numpy()),
+                lambda: tempo_amd.gated_recurrence(None)):
+        with pytest.raises(TypeError):
+            bad()
